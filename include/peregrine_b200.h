@@ -237,6 +237,71 @@ int coli_cuda_moe_layer_set_bias(ColiCudaMoeLayer *layer, const float *router_bi
 int coli_cuda_pipe_embed(int device, float *x_dev, const float *table_dev, const int *ids_dev, int S, int D, int V);
 int coli_cuda_pipe_argmax(int device, int *ids_dev, const float *logits_dev, int S, int V);
 
+/* ---- the attention half of a decode layer (no counterpart in cuda/backend_cuda.h, whose attention entry
+ * points are MLA on fp32 latents).  Device pointers, enqueued on the device's stream with no host
+ * synchronisation and no allocation, so all three can be recorded into a graph; the caller's current device
+ * is left as it was.  A refused call prints the reason, launches nothing and returns 0.
+ *
+ * ColiCudaKv names one layer's cache of keys and values: element (sequence, kv head, slot, d) of k and v is at
+ * sequence * seq_stride + head * head_stride + slot * slot_stride + d (strides in elements, multiples of 8;
+ * all three 0: dense [n_seq, n_kv, cap, D]); k and v 16-byte aligned, 1 <= n_kv, 1 <= n_seq, 1 <= cap, D one of
+ * 64, 128, 256; dtype 1 = bf16, 2 = f16.  pos and acc are dense [n_seq, n_kv, cap] or NULL: the position each
+ * slot was stored with, and the attention weight it has received so far.  Slots that were never stored may hold
+ * anything: no result depends on them. */
+typedef struct ColiCudaKv {
+    void *k, *v;
+    int32_t *pos;
+    float *acc;
+    int n_seq, n_kv, cap, D, dtype;
+    long long seq_stride, head_stride, slot_stride;
+} ColiCudaKv;
+
+/* Norms of queries and keys per head, rotation of both and the store into the cache, in one pass.
+ * qkv_dev: fp32 rows [S, row_stride] (16-byte aligned, row_stride a multiple of 4) holding H query heads, n_kv
+ * key heads and n_kv value heads of D floats.  Rows come in n_seq runs of rows_per_seq (S = n_seq *
+ * rows_per_seq): row i of sequence b goes to slot base_dev[b] + i; a slot at or past cap is not stored (q is
+ * still written), and a sequence with base_dev[b] < 0 is padding, nothing of it is written.
+ * Per q and k head: y = x * rsqrt(mean(x^2) + eps) * w (q_w / k_w fp32 [D], NULL = no norm), then the first
+ * R dims (even, 0 <= R <= D) turn by pos_dev[s] * theta^(-2j/R) (angles in 64 bits): style 0 takes
+ * pairs (2j, 2j+1) to (j, R/2 + j) as coli_cuda_pipe_rope does, style 1 pairs (j, R/2 + j) in place.  Values
+ * are stored as they are.  q_out [S, H, D] has the cache's dtype; kv->pos receives pos_dev[s] and kv->acc zero
+ * at the stored slots. */
+int coli_cuda_pipe_qk_norm_rope(int device, void *q_out, const float *qkv_dev, long long row_stride, int S, int H,
+                                const ColiCudaKv *kv, const float *q_w, const float *k_w, float eps,
+                                const int *pos_dev, const int *base_dev, int rows_per_seq, float theta, int R,
+                                int style);
+
+/* Attention of n_seq sequences that share the first prefix_len slots of `prefix` (one sequence; NULL with
+ * prefix_len 0) and each have slots of their own behind it.  q [S, H, D] of the cache's dtype, H a multiple
+ * of n_kv (query head h reads kv head h / (H / n_kv)), rows in runs of rows_per_seq (1..64) as above, their own keys
+ * already stored at base_dev[b] + i.  Row i sees the prefix, its sequence's slots below base_dev[b], and of the
+ * new slots base_dev[b] + j those with bit j of mask_dev[s] set (mask_dev NULL: j <= i); never a slot at or
+ * past own->cap.  out [S, H, D] = softmax(scale q.k) v over what the row sees, fp32 (out_f32 = 1) or the cache's
+ * dtype (0); a row that sees nothing is 0; rows of a sequence with base_dev[b] < 0 are left as they were.
+ * When own->acc is set, acc[b, kv head, slot] grows by the softmax weights the slot received from the rows and
+ * heads of its group.  Products of 16-bit values are summed in fp32, softmax statistics are fp32, and with
+ * out_f32 the weights enter the second product with at least 22 bits (the dtype's own precision otherwise).
+ * Results do not change from run to run.  work_dev: scratch of the caller's, at least
+ * coli_cuda_pipe_attention_workspace(...) bytes, 256-byte aligned; calls that may overlap on the GPU need one each. */
+int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, const void *q_dev, int S, int H,
+                             const ColiCudaKv *prefix, int prefix_len, const ColiCudaKv *own, const int *base_dev,
+                             int rows_per_seq, const uint64_t *mask_dev, float scale, void *work_dev,
+                             size_t work_bytes);
+/* Bytes of work_dev for a call with these arguments (0: the call would be refused). */
+size_t coli_cuda_pipe_attention_workspace(int device, int S, int H, const ColiCudaKv *own, int prefix_len,
+                                          int rows_per_seq);
+
+/* Keeps at most `keep` slots of every (sequence, kv head) of `src`, which has len_dev[b] slots in use (more than
+ * cap counts as cap), and writes them to `dst` (same n_seq, n_kv, D, dtype; cap >= keep; pos and acc set in both).
+ * Rank: first the protected slots, pos < sinks or pos > last - recent with last the largest position in use;
+ * then by acc, larger first (NaN last, +0 = -0); ties to the lower slot.  Kept slots below min(keep, len) stay
+ * where they are, and the m-th slot below it that is not kept receives the m-th kept slot from behind: no order
+ * beyond that.  dst may be src itself, which then moves only the latter.  index_dev [n_seq, n_kv, keep]: the
+ * source slot of every kept one, -1 behind them.  new_len_dev[b] = min(len_dev[b], keep) (may be len_dev itself).
+ * Sequences with len_dev[b] < 0 are padding: nothing of them but new_len_dev[b] (= len_dev[b]) is written. */
+int coli_cuda_pipe_kv_evict(int device, const ColiCudaKv *dst, const ColiCudaKv *src, const int *len_dev,
+                            int *new_len_dev, int *index_dev, int keep, int sinks, int recent);
+
 /* Expert parallelism over the GPUs of one node (the reference has none: crates/peregrine-model/src/gpu.rs:1454-1457
  * hard-codes one device; docs/scale-out-design.md:34-72 sketches an owner map per (layer, expert) and requires
  * cross-device partial sums in fixed order).  Rank r of `world` owns the routed experts

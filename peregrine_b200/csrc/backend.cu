@@ -17,6 +17,7 @@
 #include "kernels_fold.cuh"
 #include "kernels_decode.cuh"
 #include "kernels_ep.cuh"
+#include "ctx.h"
 #include "w4_host.h"
 
 using namespace pgb;
@@ -176,6 +177,18 @@ static int ensure_smem(Ctx *c, K kernel, size_t bytes, const char *what) {
     tab.push_back({fn, (int)bytes});
     return 1;
 }
+
+// What the other translation units need of a context (ctx.h).
+int pgb::ctx_of(int device, CtxRef *ref) {
+    Ctx *c = find_ctx(device);
+    if (!c || c->device < 0) return 0;
+    ref->device = c->device;
+    ref->stream = c->stream;
+    ref->sms = c->sms;
+    ref->err = c->err_dev;
+    return 1;
+}
+void pgb::count_launches(int n) { g_launches.fetch_add((uint64_t)n, std::memory_order_relaxed); }
 
 PGB_EXPORT int coli_cuda_probe_device_count(void) {
     int n = 0;

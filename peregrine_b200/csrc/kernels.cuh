@@ -8,52 +8,10 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "ptx.cuh"
 #include "w4_layout.h"
 
 namespace pgb {
-
-// ------------------------------------------------------------------ PTX glue
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok;
-}
-// 1-D bulk copy global -> shared (TMA engine), completion counted on an mbarrier.
-// Source, destination and size must be multiples of 16 bytes.  One destination CTA.
-__device__ __forceinline__ void bulk_g2s(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
-}
-// Programmatic dependent launch: a launch made with the programmatic-serialisation attribute may
-// start while its predecessor in the stream is still running; it must not touch anything the
-// predecessor writes before griddep_wait().  Both are no-ops in an ordinary launch.
-__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void griddep_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-// Bulk prefetch of a global range into L2 (source 16-byte aligned, size a multiple of 16 bytes).
-__device__ __forceinline__ void bulk_prefetch_l2(const void *src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void fence_mbar_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 
 // unsigned bytes of `a` times signed bytes of `b`, accumulated into c
 __device__ __forceinline__ int dp4a_us(uint32_t a, uint32_t b, int c) {
@@ -68,15 +26,6 @@ __device__ __forceinline__ float exp32(float v) { return __double2float_rn(exp((
 // crates/peregrine-model/src/math.rs:103-110
 __device__ __forceinline__ float sigmoid32(float v) { return __fdiv_rn(1.0f, __fadd_rn(1.0f, exp32(-v))); }
 __device__ __forceinline__ float silu32(float v) { return __fdiv_rn(v, __fadd_rn(1.0f, exp32(-v))); }
-
-// The per-device error word lives in page-locked host memory that the device can address, so the
-// host reads it after a synchronise without queueing a copy.  It is only written on a failure.
-__device__ __forceinline__ void report_error(int *err, int code) {
-    *reinterpret_cast<volatile int *>(err) = code;
-    __threadfence_system();
-}
-// Error codes written to the per-device error word.
-enum : int { kErrNone = 0, kErrBarrierTimeout = 1 };
 
 // ------------------------------------------------------- activation quantiser
 // Layout of the quantised activations a launch consumes.

@@ -22,21 +22,6 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
         : "memory");
 }
-// One thread of a converged warp, chosen in the form that the compiler knows to be a single one: an MMA pair with its
-// commits takes 34 cycles to issue in a block chosen by elect.sync and 165 under a condition like `lane == 0`
-// (measured; bulk and tensor copies are of the same kind).
-__device__ __forceinline__ bool elect_one() {
-    uint32_t p;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-    return p != 0;
-}
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
 // try_wait that lets the hardware park the thread for up to `ns` nanoseconds instead of
 // returning at once (the peak probe, whose MMAs run for long)
 __device__ __forceinline__ uint32_t mbar_try_wait_park(uint32_t bar, uint32_t parity, uint32_t ns) {
@@ -49,37 +34,6 @@ __device__ __forceinline__ uint32_t mbar_try_wait_park(uint32_t bar, uint32_t pa
         : "r"(bar), "r"(parity), "r"(ns)
         : "memory");
     return ok;
-}
-
-// bounded wait that also gives up when another role has already failed
-__device__ __forceinline__ bool um_wait(uint32_t bar, uint32_t parity, volatile int *fail) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
-        if (*fail) return false;
-        if (clock64() - t0 > 2000000000LL) {
-            *fail = 1;
-            return false;
-        }
-    }
-    return true;
-}
-
-// Arrival of lane 0 of a warp, without a branch
-__device__ __forceinline__ void mbar_arrive_lane0(uint32_t bar, int lane) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.eq.s32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar),
-                 "r"(lane)
-                 : "memory");
-}
-// The same for loops that go on after a failure: the waits that follow return at once (the flag is set), the
-// accesses stay in bounds, the results are reported as bad.  Saves the vote of every single wait.
-__device__ __forceinline__ void um_spin(uint32_t bar, uint32_t parity, volatile int *fail) {
-    if (mbar_try_wait(bar, parity)) return;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
-        if (*fail) return;
-        if (clock64() - t0 > 2000000000LL) *fail = 1;
-    }
 }
 
 // ---------------------------------------------------------------- int8 tensor peak probe

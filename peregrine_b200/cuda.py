@@ -49,7 +49,9 @@ SYMBOLS = [
     "coli_cuda_ep_attach_ptr", "coli_cuda_ep_free", "coli_cuda_ep_reset", "coli_cuda_moe_layer_ep_route_dev",
     "coli_cuda_moe_layer_ep_dispatch_dev", "coli_cuda_moe_layer_ep_experts_dev", "coli_cuda_moe_layer_ep_finish_dev",
     "coli_cuda_moe_layer_ep_forward_dev", "coli_cuda_moe_layer_set_profile", "coli_cuda_moe_layer_profile",
-    "coli_cuda_pipe_gemm_noalloc", "coli_cuda_pipe_embed", "coli_cuda_pipe_argmax", "coli_cuda_last_device_error", "coli_cuda_selftest_bounded_wait", "coli_cuda_kernel_launches", "coli_cuda_stream",
+    "coli_cuda_pipe_gemm_noalloc", "coli_cuda_pipe_embed", "coli_cuda_pipe_argmax",
+    "coli_cuda_pipe_qk_norm_rope", "coli_cuda_pipe_attention", "coli_cuda_pipe_attention_workspace",
+    "coli_cuda_pipe_kv_evict", "coli_cuda_last_device_error", "coli_cuda_selftest_bounded_wait", "coli_cuda_kernel_launches", "coli_cuda_stream",
 ]
 
 
