@@ -90,17 +90,66 @@ struct NormRopeLaunch {
     }
 };
 
+int row_tile(long long m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
+
+// CTAs of the split kernel: as many as are resident at once (shared memory of a CTA: 73, 113 or 193 kB).
+int attn_ctas(int D, int sms) { return sms * (D == 64 ? 3 : D == 128 ? 2 : 1); }
+
+// Shapes and the scratch's layout from the description of a call; bytes needed, or 0 for numbers past the kernels' range.
+size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, int rows, int sms, char *work) {
+    const long long m_own = (long long)rows * (H / own.n_kv), m_pre = (long long)S * (H / own.n_kv);
+    P->G = H / own.n_kv;
+    P->rt_own = row_tile(m_own);
+    P->rt_pre = row_tile(m_pre);
+    P->rt_max = prefix_len ? (P->rt_pre > P->rt_own ? P->rt_pre : P->rt_own) : P->rt_own;
+    const long long mt_own = (m_own + P->rt_own - 1) / P->rt_own, mt_pre = prefix_len ? (m_pre + P->rt_pre - 1) / P->rt_pre : 0;
+    const long long units = own.n_kv * (mt_pre + own.n_seq * mt_own);
+    if (units > 0x3fffffff || m_pre > 0x3fffffff) return 0;
+    P->mt_own = (int)mt_own;
+    P->mt_pre = (int)mt_pre;
+    P->ctas = attn_ctas(own.D, sms);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        char *p = work ? work + at : nullptr;
+        at += (bytes + 255) & ~(size_t)255;
+        return p;
+    };
+    const size_t rows_all = (size_t)(units + P->ctas) * P->rt_max;
+    P->part = reinterpret_cast<float *>(take(rows_all * own.D * 4));
+    P->ml = reinterpret_cast<float2 *>(take(rows_all * 8));
+    P->offs = reinterpret_cast<int *>(take(((size_t)own.n_seq + 1) * 4));
+    P->scores = own.acc ? reinterpret_cast<float *>(take((size_t)own.n_seq * own.n_kv * m_own * own.cap * 4)) : nullptr;
+    return at;
+}
+
+template <typename K>
+int opt_in(K kernel, int bytes) {  // per device and cheap: set on every launch that needs it
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    return e == cudaSuccess ? 1 : refuse("shared-memory opt-in: %s", cudaGetErrorString(e));
+}
+
 struct AttnLaunch {
     const AttnArgs &P;
     cudaStream_t stream;
     template <int D, bool BF16>
     int operator()() const {
-        attn_rows_kernel<D, BF16><<<dim3((unsigned)((long long)P.S * P.H)), 128, 0, stream>>>(P);
+        auto split = P.out_f32 ? attn_split_kernel<D, BF16, true> : attn_split_kernel<D, BF16, false>;
+        if (!opt_in(split, kAtSmem<D>)) return 0;
+        split<<<dim3(P.ctas), kAtThreads, kAtSmem<D>, stream>>>(P);
         if (!launched("attention launch")) return 0;
-        if (!P.own.acc) return 1;
-        const long long warps = (long long)P.own.n_seq * P.own.n_kv * P.own.cap;
-        attn_acc_kernel<D, BF16><<<dim3((unsigned)((warps + 7) / 8)), 256, 0, stream>>>(P);
-        return launched("attention weights launch");
+        // the joining launch starts early and waits on the device for the first one's end
+        const int chunks = P.own.acc ? (P.own.cap + 2 * kAtCombine - 1) / (2 * kAtCombine) : 0;
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = dim3((unsigned)((long long)P.S * P.H + (long long)chunks * P.own.n_seq * P.own.n_kv));
+        cfg.blockDim = dim3(kAtCombine);
+        cfg.stream = stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, attn_join_kernel<D, BF16>, P, chunks);
+        return launched("attention join launch");
     }
 };
 
@@ -149,7 +198,9 @@ PGB_EXPORT size_t coli_cuda_pipe_attention_workspace(int device, int S, int H, c
     if (!kv_args(&kv, own, what) || !rows_ok(S, H, kv, rows_per_seq, what)) return 0;
     if (prefix_len < 0 || H % kv.n_kv || rows_per_seq > 64) return (size_t)refuse("%s: shape", what);
     if (!ctx_of(device, &c)) return (size_t)refuse("%s: device %d is not initialised", what, device);
-    return (size_t)S * H * 8;
+    AttnArgs P{};
+    const size_t need = attn_plan(&P, kv, S, H, prefix_len, rows_per_seq, c.sms, nullptr);
+    return need ? need : (size_t)refuse("%s: too many rows and heads", what);
 }
 
 PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, const void *q_dev, int S, int H,
@@ -162,7 +213,8 @@ PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, 
     if (!kv_args(&P.own, own, what) || !rows_ok(S, H, P.own, rows_per_seq, what)) return 0;
     if (rows_per_seq > 64) return refuse("%s: %d rows of a sequence are more than 64", what, rows_per_seq);
     if (H % own->n_kv) return refuse("%s: %d heads are no multiple of %d", what, H, own->n_kv);
-    if ((long long)S * H > 0x7fffffffll) return refuse("%s: too many rows and heads", what);
+    if ((long long)S * H + (own->acc ? (long long)(own->cap / 256 + 1) * own->n_seq * own->n_kv : 0) > 0x7fffffffll)
+        return refuse("%s: too many rows and heads", what);
     if (!out_dev || !q_dev || !base_dev || !work_dev) return refuse("%s: null pointer", what);
     if (!aligned(out_dev, 16) || !aligned(q_dev, 16) || !aligned(base_dev, 4) || !aligned(mask_dev, 8) || !aligned(work_dev, 256))
         return refuse("%s: misaligned pointer", what);
@@ -180,16 +232,14 @@ PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, 
     P.q = static_cast<const uint16_t *>(q_dev);
     P.S = S;
     P.H = H;
-    P.G = H / own->n_kv;
     P.prefix_len = prefix_len;
     P.base = base_dev;
     P.rows = rows_per_seq;
     P.mask = reinterpret_cast<const unsigned long long *>(mask_dev);
-    P.scale = scale;
-    P.stats = static_cast<float *>(work_dev);
+    P.scale2 = scale * 1.4426950408889634f;
     if (!ctx_of(device, &c)) return refuse("%s: device %d is not initialised", what, device);
-    const size_t need = coli_cuda_pipe_attention_workspace(device, S, H, own, prefix_len, rows_per_seq);
-    if (!need) return 0;
+    const size_t need = attn_plan(&P, P.own, S, H, prefix_len, rows_per_seq, c.sms, static_cast<char *>(work_dev));
+    if (!need) return refuse("%s: too many rows and heads", what);
     if (work_bytes < need) return refuse("%s: %zu bytes of workspace, %zu are needed", what, work_bytes, need);
     DeviceGuard g(c.device);
     if (!g.ok()) return refuse("%s: device %d cannot be selected", what, device);
