@@ -6,7 +6,7 @@
 
 #include "../../include/peregrine_b200.h"
 #include "ctx.h"
-#include "kernels_attn.cuh"
+#include "kernels_attn_tc.cuh"
 #include "kernels_evict.cuh"
 #include "kernels_norm_rope.cuh"
 
@@ -95,8 +95,11 @@ int row_tile(long long m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
 // CTAs of the split kernel: as many as are resident at once (shared memory of a CTA: 73, 113 or 193 kB).
 int attn_ctas(int D, int sms) { return sms * (D == 64 ? 3 : D == 128 ? 2 : 1); }
 
+// Problems with more row vectors than this go to the tensor-memory kernel, whose tiles have 128 rows.
+constexpr int kTcRows = 32;
+
 // Shapes and the scratch's layout from the description of a call; bytes needed, or 0 for numbers past the kernels' range.
-size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, int rows, int sms, char *work) {
+size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, int rows, bool wide_weights, int sms, char *work) {
     const long long m_own = (long long)rows * (H / own.n_kv), m_pre = (long long)S * (H / own.n_kv);
     P->G = H / own.n_kv;
     P->rt_own = row_tile(m_own);
@@ -108,6 +111,16 @@ size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, i
     P->mt_own = (int)mt_own;
     P->mt_pre = (int)mt_pre;
     P->ctas = attn_ctas(own.D, sms);
+    P->tc_keys = own.D == 256 || wide_weights ? 64 : 128;
+    P->tc_rows = own.D == 256 ? 128 : 256;
+    P->tc_ctas = sms;
+    P->tc_pre = m_pre > kTcRows && prefix_len >= P->tc_keys;
+    P->tc_own = m_own > kTcRows && own.cap >= P->tc_keys;
+    P->cut_pre = P->tc_pre ? prefix_len / P->tc_keys * P->tc_keys : 0;
+    P->tc2_pre = own.D < 256 && m_pre <= 128;
+    P->tc2_own = own.D < 256 && m_own <= 128;
+    P->tcm_pre = P->tc_pre ? (int)((m_pre + P->tc_rows - 1) / P->tc_rows) : 0;
+    P->tcm_own = P->tc_own ? (int)((m_own + P->tc_rows - 1) / P->tc_rows) : 0;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         char *p = work ? work + at : nullptr;
@@ -119,7 +132,38 @@ size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, i
     P->ml = reinterpret_cast<float2 *>(take(rows_all * 8));
     P->offs = reinterpret_cast<int *>(take(((size_t)own.n_seq + 1) * 4));
     P->scores = own.acc ? reinterpret_cast<float *>(take((size_t)own.n_seq * own.n_kv * m_own * own.cap * 4)) : nullptr;
+    if (P->tc_pre || P->tc_own) {
+        const size_t tc_all = ((size_t)own.n_kv * (P->tcm_pre + (size_t)own.n_seq * P->tcm_own) + P->tc_ctas) * P->tc_rows;
+        P->tc_part = reinterpret_cast<float *>(take(tc_all * own.D * 4));
+        P->tc_ml = reinterpret_cast<float2 *>(take(tc_all * 8));
+        P->tc_offs = reinterpret_cast<int *>(take(((size_t)own.n_seq + 1) * 4));
+    }
     return at;
+}
+
+// Copies of [keys][64 dims] boxes of a cache, swizzled by 128 bytes.
+int kv_map(CUtensorMap *m, const void *p, const KvArgs &kv, int dtype, int keys) {
+    typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const EncodeFn enc = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult st;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &st) != cudaSuccess || st != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            fn = nullptr;
+        }
+        return (EncodeFn)fn;
+    }();
+    if (!enc) return 0;
+    // a stride of a dimension with one entry is never used, but has to be a valid one
+    const long long head = kv.n_kv > 1 ? kv.head_stride : kv.slot_stride, seq = kv.n_seq > 1 ? kv.seq_stride : kv.slot_stride;
+    const cuuint64_t dims[4] = {(cuuint64_t)kv.D, (cuuint64_t)kv.cap, (cuuint64_t)kv.n_kv, (cuuint64_t)kv.n_seq};
+    const cuuint64_t strides[3] = {(cuuint64_t)kv.slot_stride * 2, (cuuint64_t)head * 2, (cuuint64_t)seq * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)keys, 1, 1}, es[4] = {1, 1, 1, 1};
+    return enc(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(p), dims, strides,
+               box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename K>
@@ -128,28 +172,52 @@ int opt_in(K kernel, int bytes) {  // per device and cheap: set on every launch 
     return e == cudaSuccess ? 1 : refuse("shared-memory opt-in: %s", cudaGetErrorString(e));
 }
 
+// A launch that may start while the one before it in the stream still runs.
+template <typename... K, typename... A>
+int launch_early(void (*kernel)(K...), unsigned grid, int block, int smem, cudaStream_t stream, const char *what, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, K(args)...);
+    return launched(what);
+}
+
 struct AttnLaunch {
     const AttnArgs &P;
+    const CUtensorMap *maps;  // of the prefix's and the own keys and values
     cudaStream_t stream;
+    template <int D, bool BF16, bool F32>
+    int run() const {
+        auto split = attn_split_kernel<D, BF16, F32>;
+        if (!opt_in(split, kAtSmem<D>)) return 0;
+        if (P.tc_pre || P.tc_own) {
+            using T = TcShape<D, BF16, F32>;
+            static_assert(T::ROWS == (D == 256 ? 128 : 256) && T::N == (D == 256 || (BF16 && F32) ? 64 : 128), "as planned");
+            auto tc = attn_tc_kernel<D, BF16, F32>;
+            if (!opt_in(tc, T::SMEM)) return 0;
+            tc<<<dim3(P.tc_ctas), T::THREADS, T::SMEM, stream>>>(P, maps[0], maps[1], maps[2], maps[3]);
+            if (!launched("attention tensor launch")) return 0;
+            // needs nothing of the one before: it fills the SMs that this leaves, and ends after it
+            if (!launch_early(split, P.ctas, kAtThreads, kAtSmem<D>, stream, "attention launch", P)) return 0;
+        } else {
+            split<<<dim3(P.ctas), kAtThreads, kAtSmem<D>, stream>>>(P);
+            if (!launched("attention launch")) return 0;
+        }
+        // waits on the device for the end of the launches before
+        const int chunks = P.own.acc ? (P.own.cap + 2 * kAtCombine - 1) / (2 * kAtCombine) : 0;
+        const unsigned grid = (unsigned)((long long)P.S * P.H + (long long)chunks * P.own.n_seq * P.own.n_kv);
+        return launch_early(attn_join_kernel<D, BF16>, grid, kAtCombine, 0, stream, "attention join launch", P, chunks);
+    }
     template <int D, bool BF16>
     int operator()() const {
-        auto split = P.out_f32 ? attn_split_kernel<D, BF16, true> : attn_split_kernel<D, BF16, false>;
-        if (!opt_in(split, kAtSmem<D>)) return 0;
-        split<<<dim3(P.ctas), kAtThreads, kAtSmem<D>, stream>>>(P);
-        if (!launched("attention launch")) return 0;
-        // the joining launch starts early and waits on the device for the first one's end
-        const int chunks = P.own.acc ? (P.own.cap + 2 * kAtCombine - 1) / (2 * kAtCombine) : 0;
-        cudaLaunchConfig_t cfg{};
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.gridDim = dim3((unsigned)((long long)P.S * P.H + (long long)chunks * P.own.n_seq * P.own.n_kv));
-        cfg.blockDim = dim3(kAtCombine);
-        cfg.stream = stream;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        cudaLaunchKernelEx(&cfg, attn_join_kernel<D, BF16>, P, chunks);
-        return launched("attention join launch");
+        return P.out_f32 ? run<D, BF16, true>() : run<D, BF16, false>();
     }
 };
 
@@ -199,7 +267,8 @@ PGB_EXPORT size_t coli_cuda_pipe_attention_workspace(int device, int S, int H, c
     if (prefix_len < 0 || H % kv.n_kv || rows_per_seq > 64) return (size_t)refuse("%s: shape", what);
     if (!ctx_of(device, &c)) return (size_t)refuse("%s: device %d is not initialised", what, device);
     AttnArgs P{};
-    const size_t need = attn_plan(&P, kv, S, H, prefix_len, rows_per_seq, c.sms, nullptr);
+    const size_t n0 = attn_plan(&P, kv, S, H, prefix_len, rows_per_seq, false, c.sms, nullptr);
+    const size_t n1 = attn_plan(&P, kv, S, H, prefix_len, rows_per_seq, true, c.sms, nullptr), need = n0 > n1 ? n0 : n1;
     return need ? need : (size_t)refuse("%s: too many rows and heads", what);
 }
 
@@ -238,12 +307,17 @@ PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, 
     P.mask = reinterpret_cast<const unsigned long long *>(mask_dev);
     P.scale2 = scale * 1.4426950408889634f;
     if (!ctx_of(device, &c)) return refuse("%s: device %d is not initialised", what, device);
-    const size_t need = attn_plan(&P, P.own, S, H, prefix_len, rows_per_seq, c.sms, static_cast<char *>(work_dev));
+    const size_t need = attn_plan(&P, P.own, S, H, prefix_len, rows_per_seq, out_f32 && own->dtype == 1, c.sms, static_cast<char *>(work_dev));
     if (!need) return refuse("%s: too many rows and heads", what);
     if (work_bytes < need) return refuse("%s: %zu bytes of workspace, %zu are needed", what, work_bytes, need);
+    P.err = c.err;
     DeviceGuard g(c.device);
     if (!g.ok()) return refuse("%s: device %d cannot be selected", what, device);
-    return by_type(own->D, own->dtype, AttnLaunch{P, c.stream});
+    CUtensorMap maps[4] = {};
+    if ((P.tc_pre && !(kv_map(&maps[0], P.pre.k, P.pre, own->dtype, P.tc_keys) && kv_map(&maps[1], P.pre.v, P.pre, own->dtype, P.tc_keys))) ||
+        (P.tc_own && !(kv_map(&maps[2], P.own.k, P.own, own->dtype, P.tc_keys) && kv_map(&maps[3], P.own.v, P.own, own->dtype, P.tc_keys))))
+        return refuse("%s: the cache's strides cannot be described to the copy engine", what);
+    return by_type(own->D, own->dtype, AttnLaunch{P, maps, c.stream});
 }
 
 PGB_EXPORT int coli_cuda_pipe_kv_evict(int device, const ColiCudaKv *dst, const ColiCudaKv *src, const int *len_dev,

@@ -31,6 +31,18 @@ struct AttnArgs {
     int ctas;                    // CTAs that share the line of tiles
     int rt_pre, rt_own, rt_max;  // rows of a row tile: 16, 32 or 64
     int mt_pre, mt_own;          // row tiles of a problem (mt_pre 0: no prefix)
+    // Tiles of tc_keys keys that every row of the problem sees, of problems with many rows, go to the tensor-memory
+    // kernel (kernels_attn_tc.cuh); this one keeps what is left: the keys from cut_pre (prefix) or own_cut (own) on.
+    int tc_keys;             // 64 or 128
+    int tc_pre, tc_own;      // whether the prefix, the own slots are split this way
+    int cut_pre;             // keys of the prefix that the tensor-memory kernel takes
+    int tc_ctas, tc_rows;    // its CTAs, rows of one of its partials
+    int tcm_pre, tcm_own;    // its row tiles of a problem
+    int tc2_pre, tc2_own;    // 1: a row tile has 128 rows and its keys go to two halves of a partial in turn
+    float *tc_part;          // [its problems x row tiles + tc_ctas][tc_rows][D]
+    float2 *tc_ml;
+    int *tc_offs;  // [n_seq + 1]: its tiles of the sequences before b
+    int *err;
     // scratch
     float *part;    // [problems x row tiles + ctas][rt_max][D]: outputs of the partials, unnormalised
     float2 *ml;     // [..][rt_max]: their m and l
@@ -52,6 +64,12 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ int own_keys(const AttnArgs &P, int b) {
     const int base = P.base[b];
     return base < 0 ? 0 : (int)min((long long)base + P.rows, (long long)P.own.cap);
+}
+// How many of them the tensor-memory kernel takes.
+__device__ __forceinline__ int own_cut(const AttnArgs &P, int b) {
+    if (!P.tc_own) return 0;
+    const int base = P.base[b];
+    return base < 0 ? 0 : min(base, P.own.cap) / P.tc_keys * P.tc_keys;
 }
 // New slots that row i of a sequence sees, a bit each.
 __device__ __forceinline__ unsigned long long row_mask(const AttnArgs &P, int row, int i) {
@@ -115,8 +133,11 @@ __device__ __forceinline__ uint32_t finite16(uint32_t v) {
 
 // A place on the line of tiles: tile `tile` of the row tile `mt` of kv head `kvh` of sequence `seq` (-1: the prefix).
 struct AttnAt {
-    int seq, kvh, mt, tile, tiles, keys;
+    int seq, kvh, mt, tile, tiles, k0, keys;  // tile t holds the keys [k0 + 64 t, ...) below `keys`
 };
+__device__ __forceinline__ int own_tiles(const AttnArgs &P, int b) {
+    return (own_keys(P, b) - own_cut(P, b) + kAtKeys - 1) / kAtKeys;
+}
 __device__ __forceinline__ void attn_step(const AttnArgs &P, AttnAt &a) {
     if (++a.tile < a.tiles) return;
     a.tile = 0;
@@ -130,8 +151,9 @@ __device__ __forceinline__ void attn_step(const AttnArgs &P, AttnAt &a) {
             return;
         }
         a.keys = own_keys(P, a.seq);
-    } while (a.keys == 0);
-    a.tiles = (a.keys + kAtKeys - 1) / kAtKeys;
+        a.k0 = own_cut(P, a.seq);
+        a.tiles = (a.keys - a.k0 + kAtKeys - 1) / kAtKeys;
+    } while (a.tiles == 0);
 }
 // Number of the (problem, row tile) on the line.
 __device__ __forceinline__ int attn_unit(const AttnArgs &P, const AttnAt &a) {
@@ -141,6 +163,63 @@ __device__ __forceinline__ int attn_unit(const AttnArgs &P, const AttnAt &a) {
 // Where CTA c's part begins.  No more CTAs share the line than it has tiles, so that no part is empty.
 __device__ __forceinline__ long long line_part(long long total, int ctas, int c) { return total * c / ctas; }
 __device__ __forceinline__ int line_ctas(long long total, int ctas) { return (int)min((long long)ctas, max(total, 1ll)); }
+
+// This CTA's part [first, end) of a line made of `line_pre` tiles of the prefix and, per sequence, tiles_of(b) * per_seq
+// own ones; `seq` and `off` (tiles of the sequences before it): the sequence of the first tile, where it is an own one.
+// CTA 0 writes the table of offsets.  False: no tile is this CTA's.  W: warps of the CTA, all of which call.
+template <int W, typename F>
+__device__ __forceinline__ bool line_share(int ns, F tiles_of, int per_seq, long long line_pre, int ctas, int *offs,
+                                           long long &first, long long &end, int &seq, int &off) {
+    __shared__ long long s_sum[W];
+    __shared__ int s_seq, s_off;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
+    long long units = 0;
+    for (int b = tid; b < ns; b += W * 32) units += tiles_of(b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
+    if (lane == 0) s_sum[warp] = units;
+    __syncthreads();
+    units = 0;
+    for (int w = 0; w < W; ++w) units += s_sum[w];
+    const long long total = line_pre + units * per_seq;
+    const int nc = line_ctas(total, ctas);
+    if (c >= nc) return false;
+    first = line_part(total, nc, c);
+    end = line_part(total, nc, c + 1);
+    if (first >= line_pre || c == 0) {
+        int run = 0;
+        for (int b0 = 0; b0 < ns; b0 += W * 32) {
+            const int b = b0 + tid, n = b < ns ? tiles_of(b) : 0;
+            int x = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            __syncthreads();
+            if (lane == 31) s_sum[warp] = x;
+            __syncthreads();
+            int at = run + x - n;
+            for (int w = 0; w < W; ++w) {
+                if (w < warp) at += (int)s_sum[w];
+                run += (int)s_sum[w];
+            }
+            if (b < ns) {
+                if (c == 0) offs[b] = at;
+                const long long lo = line_pre + (long long)at * per_seq;
+                if (n && first >= lo && first < lo + (long long)n * per_seq) {
+                    s_seq = b;
+                    s_off = at;
+                }
+            }
+        }
+        if (c == 0 && tid == 0) offs[ns] = run;
+        __syncthreads();
+        seq = s_seq;
+        off = s_off;
+    }
+    return first < end;
+}
 
 template <int D>
 constexpr int kAtStages = D == 64 ? 4 : D == 128 ? 3 : 2;
@@ -157,9 +236,8 @@ __device__ __forceinline__ void attn_load(const AttnArgs &P, const AttnAt &a, ui
     constexpr int C = D / 8, KPI = kAtThreads / C;  // 16-byte pieces of a key, keys per pass
     const KvArgs &kv = a.seq < 0 ? P.pre : P.own;
     const int c = threadIdx.x % C, k0 = threadIdx.x / C;
-    const int left = a.keys - a.tile * kAtKeys;
-    const long long at = (a.seq < 0 ? 0 : (long long)a.seq * kv.seq_stride) + a.kvh * kv.head_stride +
-                         (long long)a.tile * kAtKeys * kv.slot_stride + c * 8;
+    const int t0 = a.k0 + a.tile * kAtKeys, left = a.keys - t0;
+    const long long at = (a.seq < 0 ? 0 : (long long)a.seq * kv.seq_stride) + a.kvh * kv.head_stride + t0 * kv.slot_stride + c * 8;
     const uint16_t *k = kv.k + at, *v = kv.v + at;
 #pragma unroll
     for (int j = 0; j < kAtKeys / KPI; ++j) {
@@ -207,7 +285,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &P, const AttnAt &a, At
             mma16<BF16>(s[2 * n + 1], af, b[2], b[3]);
         }
     }
-    const int t0 = a.tile * kAtKeys + kw, col = (lane & 3) * 2;
+    const int t0 = a.k0 + a.tile * kAtKeys + kw, col = (lane & 3) * 2;
     const bool prefix = a.seq < 0;
     const int base = prefix ? a.keys : P.base[a.seq];
     const bool open = t0 + KPW <= min(base, a.keys);  // every row sees every key of the range
@@ -348,70 +426,34 @@ template <int D, bool BF16, bool F32>
 __global__ void __launch_bounds__(kAtThreads) attn_split_kernel(const AttnArgs P) {
     extern __shared__ __align__(128) uint8_t at_smem[];
     constexpr int NS = kAtStages<D>, TB = kAtTileBytes<D>, MR = kAtMergeRow<D>;
-    __shared__ long long s_sum[4];
-    __shared__ int s_seq, s_off;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
     griddep_launch_dependents();
-    const int nkv = P.own.n_kv, ns = P.own.n_seq;
-    // ---- this CTA's part of the line
-    const int tp = P.mt_pre ? (P.prefix_len + kAtKeys - 1) / kAtKeys : 0;
-    long long units = 0;
-    for (int b = tid; b < ns; b += kAtThreads) units += (own_keys(P, b) + kAtKeys - 1) / kAtKeys;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
-    if (lane == 0) s_sum[warp] = units;
-    __syncthreads();
-    units = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-    const int per_seq = nkv * P.mt_own;
-    const long long line_pre = (long long)nkv * P.mt_pre * tp, total = line_pre + units * per_seq;
-    const int c = blockIdx.x, nc = line_ctas(total, P.ctas);
-    if (c >= nc) return;
-    const long long first = line_part(total, nc, c), end = line_part(total, nc, c + 1);
-    // the sequence that the first tile belongs to; CTA 0 writes the table of all
-    if (first >= line_pre || c == 0) {
-        int run = 0;
-        for (int b0 = 0; b0 < ns; b0 += kAtThreads) {
-            const int b = b0 + tid;
-            const int n = b < ns ? (own_keys(P, b) + kAtKeys - 1) / kAtKeys : 0;
-            int x = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            __syncthreads();
-            if (lane == 31) s_sum[warp] = x;
-            __syncthreads();
-            int off = run + x - n;
-            for (int w = 0; w < warp; ++w) off += (int)s_sum[w];
-            run += (int)(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
-            if (b < ns) {
-                if (c == 0) P.offs[b] = off;
-                const long long lo = line_pre + (long long)off * per_seq;
-                if (n && first >= lo && first < lo + (long long)n * per_seq) {
-                    s_seq = b;
-                    s_off = off;
-                }
-            }
-        }
-        if (c == 0 && tid == 0) P.offs[ns] = run;
-        __syncthreads();
+    const int nkv = P.own.n_kv, per_seq = nkv * P.mt_own;
+    const int tp = P.mt_pre ? (P.prefix_len - P.cut_pre + kAtKeys - 1) / kAtKeys : 0;
+    const long long line_pre = (long long)nkv * P.mt_pre * tp;
+    long long first, end;
+    int seq = 0, off = 0;
+    if (!line_share<kAtThreads / 32>(P.own.n_seq, [&](int b) { return own_tiles(P, b); }, per_seq, line_pre, P.ctas, P.offs, first, end,
+                                     seq, off)) {
+        griddep_wait();
+        return;
     }
-    if (first >= end) return;  // nothing to do at all
     AttnAt at;
     if (first < line_pre) {
         at.seq = -1;
         at.keys = P.prefix_len;
+        at.k0 = P.cut_pre;
         at.tiles = tp;
         const int u = (int)(first / tp);
         at.kvh = u / P.mt_pre;
         at.mt = u % P.mt_pre;
         at.tile = (int)(first % tp);
     } else {
-        at.seq = s_seq;
-        at.keys = own_keys(P, at.seq);
-        at.tiles = (at.keys + kAtKeys - 1) / kAtKeys;
-        const long long in = first - line_pre - (long long)s_off * per_seq;
+        at.seq = seq;
+        at.keys = own_keys(P, seq);
+        at.k0 = own_cut(P, seq);
+        at.tiles = own_tiles(P, seq);
+        const long long in = first - line_pre - (long long)off * per_seq;
         const int u = (int)(in / at.tiles);
         at.kvh = u / P.mt_own;
         at.mt = u % P.mt_own;
@@ -572,6 +614,7 @@ __global__ void __launch_bounds__(kAtThreads) attn_split_kernel(const AttnArgs P
         }
         attn_step(P, at);
     }
+    griddep_wait();  // the joining launch waits for this one alone, and needs the tensor-memory kernel's results too
 }
 
 // Partials of one (problem, row tile): those of the CTAs whose parts meet its stretch [u0, u1) of the line.
@@ -591,29 +634,67 @@ __device__ __forceinline__ AttnParts attn_parts(int unit, long long u0, long lon
     r.n = b - a + 1;
     return r;
 }
-// The two lists of partials of row vector r (within its sequence) of a (sequence, kv head), and its row in their tiles.
+// The lists of partials of row vector r (within its sequence) of a (sequence, kv head): of the prefix and its own slots,
+// from this kernel (0, 1) and from the tensor-memory kernel (2, 3).
 struct AttnRowParts {
-    AttnParts pre, own;
-    int pre_row, own_row;
+    AttnParts list[4];
+    int row[4], n;
 };
 __device__ __forceinline__ AttnRowParts attn_row_parts(const AttnArgs &P, int seq, int kvh, int r) {
     AttnRowParts R;
-    const int nkv = P.own.n_kv, per_seq = nkv * P.mt_own;
-    const int tp = P.mt_pre ? (P.prefix_len + kAtKeys - 1) / kAtKeys : 0;
-    const long long line_pre = (long long)nkv * P.mt_pre * tp, total = line_pre + (long long)P.offs[P.own.n_seq] * per_seq;
-    const int nc = line_ctas(total, P.ctas), rp = seq * P.rows * P.G + r;
-    R.pre_row = rp % P.rt_pre;
-    R.own_row = r % P.rt_own;
-    const int up = kvh * P.mt_pre + rp / P.rt_pre;
-    R.pre = attn_parts(up, (long long)up * tp, P.mt_pre ? (long long)(up + 1) * tp : 0, total, nc);
-    const int off = P.offs[seq], tiles = P.offs[seq + 1] - off, uo = kvh * P.mt_own + r / P.rt_own;
-    const long long lo = line_pre + (long long)off * per_seq + (long long)uo * tiles;
-    R.own = attn_parts(nkv * P.mt_pre + seq * per_seq + uo, lo, lo + tiles, total, nc);
+    const int nkv = P.own.n_kv, rp = seq * P.rows * P.G + r;
+    {
+        const int per_seq = nkv * P.mt_own, tp = P.mt_pre ? (P.prefix_len - P.cut_pre + kAtKeys - 1) / kAtKeys : 0;
+        const long long line_pre = (long long)nkv * P.mt_pre * tp, total = line_pre + (long long)P.offs[P.own.n_seq] * per_seq;
+        const int nc = line_ctas(total, P.ctas);
+        const int up = kvh * P.mt_pre + rp / P.rt_pre;
+        R.row[0] = rp % P.rt_pre;
+        R.list[0] = attn_parts(up, (long long)up * tp, P.mt_pre ? (long long)(up + 1) * tp : 0, total, nc);
+        const int off = P.offs[seq], tiles = P.offs[seq + 1] - off, uo = kvh * P.mt_own + r / P.rt_own;
+        const long long lo = line_pre + (long long)off * per_seq + (long long)uo * tiles;
+        R.row[1] = r % P.rt_own;
+        R.list[1] = attn_parts(nkv * P.mt_pre + seq * per_seq + uo, lo, lo + tiles, total, nc);
+    }
+    R.list[2] = R.list[3] = AttnParts{0, 0, 0};
+    R.row[2] = R.row[3] = 0;
+    if (P.tc_pre || P.tc_own) {
+        const int per_seq = nkv * P.tcm_own, tp = P.tc_pre ? P.cut_pre / P.tc_keys : 0;
+        const long long line_pre = (long long)nkv * P.tcm_pre * tp, total = line_pre + (long long)P.tc_offs[P.own.n_seq] * per_seq;
+        const int nc = line_ctas(total, P.tc_ctas);
+        if (P.tc_pre) {
+            const int rt = P.tc2_pre ? 128 : P.tc_rows, up = kvh * P.tcm_pre + rp / rt;
+            R.row[2] = rp % rt;
+            R.list[2] = attn_parts(up, (long long)up * tp, (long long)(up + 1) * tp, total, nc);
+            R.list[2].n <<= P.tc2_pre;
+        }
+        if (P.tc_own) {
+            const int rt = P.tc2_own ? 128 : P.tc_rows, uo = kvh * P.tcm_own + r / rt;
+            const int off = P.tc_offs[seq], tiles = P.tc_offs[seq + 1] - off;
+            const long long lo = line_pre + (long long)off * per_seq + (long long)uo * tiles;
+            R.row[3] = r % rt;
+            R.list[3] = attn_parts(nkv * P.tcm_pre + seq * per_seq + uo, lo, lo + tiles, total, nc);
+            R.list[3].n <<= P.tc2_own;
+        }
+    }
+    R.n = R.list[0].n + R.list[1].n + R.list[2].n + R.list[3].n;
     return R;
 }
-__device__ __forceinline__ long long attn_part_row(const AttnArgs &P, const AttnRowParts &R, int j) {
-    return j < R.pre.n ? (long long)(R.pre.unit + R.pre.c0 + j) * P.rt_max + R.pre_row
-                       : (long long)(R.own.unit + R.own.c0 + j - R.pre.n) * P.rt_max + R.own_row;
+// Partial j of the row vector: its statistics and, in units of D floats, its output.
+__device__ __forceinline__ const float2 *attn_part(const AttnArgs &P, const AttnRowParts &R, int j, const float *&out, int D) {
+    const int n0 = R.list[0].n, n1 = n0 + R.list[1].n, n2 = n1 + R.list[2].n;
+    if (j < n1) {
+        const bool o = j >= n0;
+        const long long at = (long long)(o ? R.list[1].unit + R.list[1].c0 + j - n0 : R.list[0].unit + R.list[0].c0 + j) * P.rt_max +
+                             (o ? R.row[1] : R.row[0]);
+        out = P.part + at * D;
+        return P.ml + at;
+    }
+    const bool o = j >= n2;
+    const int i = o ? j - n2 : j - n1, two = o ? P.tc2_own : P.tc2_pre;  // two halves of a partial follow one another
+    const long long at = (long long)((o ? R.list[3].unit + R.list[3].c0 : R.list[2].unit + R.list[2].c0) + (i >> two)) * P.tc_rows +
+                         (o ? R.row[3] : R.row[2]) + (two && (i & 1) ? 128 : 0);
+    out = P.tc_part + at * D;
+    return P.tc_ml + at;
 }
 
 // Joins the partials: CTAs [0, S x H) one row vector each; with acc, further CTAs 256 slots of one (sequence, kv head) each.
@@ -628,9 +709,10 @@ __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P,
         const int row = blockIdx.x / P.H, h = blockIdx.x % P.H, seq = row / P.rows, kvh = h / P.G;
         if (P.base[seq] < 0) return;
         const AttnRowParts R = attn_row_parts(P, seq, kvh, (row % P.rows) * P.G + h % P.G);
-        const int n = R.pre.n + R.own.n;
+        const int n = R.n;
+        const float *src;
         float m = -INFINITY;
-        for (int j = threadIdx.x; j < n; j += kAtCombine) m = fmaxf(m, P.ml[attn_part_row(P, R, j)].x);
+        for (int j = threadIdx.x; j < n; j += kAtCombine) m = fmaxf(m, attn_part(P, R, j, src, D)->x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         if (lane == 0) s_m[warp] = m;
@@ -640,11 +722,10 @@ __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P,
         float o[E] = {}, l = 0.0f;
 #pragma unroll 4
         for (int j = warp; j < n; j += 4) {
-            const long long at = attn_part_row(P, R, j);
-            const float2 ml = P.ml[at];
+            const float2 ml = *attn_part(P, R, j, src, D);
             const float f = ex2(ml.x - m);
             l = fmaf(ml.y, f, l);
-            const float *src = P.part + at * D + lane * E;
+            src += lane * E;
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
                 const float2 v = *reinterpret_cast<const float2 *>(src + e);
@@ -682,14 +763,15 @@ __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P,
         __syncthreads();
         for (int r = r0 + warp; r < min(M, r0 + 64); r += 4) {
             const AttnRowParts R = attn_row_parts(P, seq, kvh, r);
-            const int n = R.pre.n + R.own.n;
+            const int n = R.n;
+            const float *src;
             float m = -INFINITY, l = 0.0f;
-            for (int j = lane; j < n; j += 32) m = fmaxf(m, P.ml[attn_part_row(P, R, j)].x);
+            for (int j = lane; j < n; j += 32) m = fmaxf(m, attn_part(P, R, j, src, D)->x);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             if (m == -INFINITY) m = 0.0f;
             for (int j = lane; j < n; j += 32) {
-                const float2 ml = P.ml[attn_part_row(P, R, j)];
+                const float2 ml = *attn_part(P, R, j, src, D);
                 l = fmaf(ml.y, ex2(ml.x - m), l);
             }
 #pragma unroll

@@ -1,0 +1,376 @@
+// Attention of problems with many row vectors (a prefix under a whole batch, a prompt chunk) on the tensor-memory units.
+//
+// A CTA holds two tiles of 128 query vectors in shared memory and streams tiles of keys and values past them:
+//     S = Q K^T (tensor memory) -> weights 2^(x - m), written over S as the A operand -> O += P V (tensor memory)
+// One thread of a softmax warp owns one row (its TMEM lane), so a row's maximum and sum need no exchange.  The two tiles
+// alternate: while one's weights are formed the tensor unit works for the other.  A 128 x 128 tile takes the tensor unit
+// 2 x 512 cycles (D = 128) and the exponential unit (16 a cycle) 1024, so neither can wait for the other.  O is rescaled
+// only when a row's maximum has grown by 2^4 since it was last set: m only has to keep weights in range, and cancels in
+// O / l.  With at most 128 row vectors both tiles hold the same ones and the key tiles go to them in turn.  D = 256 has
+// no room for a second O: there one tile alternates between two S.
+//
+// Only key tiles that every row sees come here (kernels_attn.cuh has the rest), so there are no masks, and every copy is in
+// bounds.  Work is dealt out like there: one line of key tiles, equal parts.
+#pragma once
+#include "kernels_attn.cuh"
+
+namespace pgb {
+
+template <int D, bool BF16, bool F32>
+struct TcShape {
+    static constexpr int TILES = D == 256 ? 1 : 2;    // row tiles of a CTA, a softmax warpgroup each
+    static constexpr int BUFS = D == 256 ? 2 : 1;     // S buffers of a row tile
+    static constexpr int TERMS = kAtTerms<BF16, F32>;
+    static constexpr int N = D == 256 || TERMS == 3 ? 64 : 128;  // keys of a tile
+    // A buffer has 128 columns.  32 keys of weights take 16 columns a term; three terms outgrow the S they replace,
+    // which then sits in the upper half.
+    static constexpr int S_COL = TERMS == 3 ? 64 : 0;
+    static constexpr int O_COL = TILES * BUFS * 128;
+    static constexpr int Q_BYTES = 128 * D * 2, TILE_BYTES = N * D * 2;
+    static constexpr int FIT = (232448 - 3072 - TILES * Q_BYTES) / TILE_BYTES;
+    static constexpr int SLOTS = FIT > 12 ? 12 : FIT;
+    static constexpr int SMEM = 1024 + TILES * Q_BYTES + SLOTS * TILE_BYTES;
+    static constexpr int THREADS = TILES * 128 + 64;
+    static constexpr int ROWS = TILES * 128;
+};
+
+struct TcAt {
+    int seq, kvh, mt, tile, tiles;
+};
+__device__ __forceinline__ int tc_tiles(const AttnArgs &P, int b) { return own_cut(P, b) / P.tc_keys; }
+// Moves to the next (problem, row tile) with tiles.
+__device__ __forceinline__ void tc_next(const AttnArgs &P, TcAt &a) {
+    a.tile = 0;
+    if (++a.mt < (a.seq < 0 ? P.tcm_pre : P.tcm_own)) return;
+    a.mt = 0;
+    if (++a.kvh < P.own.n_kv) return;
+    a.kvh = 0;
+    do {
+        if (++a.seq >= P.own.n_seq) {
+            a.seq = P.own.n_seq - 1;
+            return;
+        }
+        a.tiles = tc_tiles(P, a.seq);
+    } while (a.tiles == 0);
+}
+
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {  // 128-byte swizzle, 8-row groups 1024 bytes apart
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// `i`-th user of a ring of n: its place and the parity of its turn.
+template <int n>
+struct RingAt {
+    int i = 0;
+    uint32_t ph = 0;
+    __device__ __forceinline__ void skip(int k) {
+        i += k;
+        while (i >= n) {
+            i -= n;
+            ph ^= 1u;
+        }
+    }
+};
+
+template <int D, bool BF16, bool F32>
+__global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
+    attn_tc_kernel(const AttnArgs P, const __grid_constant__ CUtensorMap pre_k, const __grid_constant__ CUtensorMap pre_v,
+                   const __grid_constant__ CUtensorMap own_k, const __grid_constant__ CUtensorMap own_v) {
+    using T = TcShape<D, BF16, F32>;
+    constexpr int N = T::N, DB = D / 64;
+    extern __shared__ __align__(128) uint8_t tc_smem_raw[];
+    __shared__ __align__(8) unsigned long long s_bar[2 * T::SLOTS + 3 * T::TILES + 2 * T::TILES * T::BUFS];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_fail;
+    const int tid = threadIdx.x, warp = tid >> 5, c = blockIdx.x;
+    griddep_launch_dependents();
+    if (tid == 0) s_fail = 0;
+    const int nkv = P.own.n_kv, per_seq = nkv * P.tcm_own, tp = P.tc_pre ? P.cut_pre / N : 0;
+    const long long line_pre = (long long)nkv * P.tcm_pre * tp;
+    long long first, end;
+    int seq = 0, off = 0;
+    if (!line_share<T::THREADS / 32>(P.own.n_seq, [&](int b) { return tc_tiles(P, b); }, per_seq, line_pre, P.tc_ctas, P.tc_offs, first,
+                                     end, seq, off))
+        return;
+    uint8_t *base = tc_smem_raw + ((1024 - (smem_u32(tc_smem_raw) & 1023)) & 1023);
+    const uint32_t q_s = smem_u32(base), ring_s = q_s + T::TILES * T::Q_BYTES;
+    const uint32_t full = smem_u32(s_bar), empty = full + 8 * T::SLOTS, qfull = empty + 8 * T::SLOTS, odone = qfull + 8 * T::TILES,
+                   sfull = odone + 8 * T::TILES, pfull = sfull + 8 * T::TILES * T::BUFS,
+                   pvdone = pfull + 8 * T::TILES * T::BUFS;
+    volatile int *fail = &s_fail;
+    if (tid == 0) {
+        for (int i = 0; i < 2 * T::SLOTS; ++i) mbar_init(full + 8 * i, 1);
+        for (int i = 0; i < T::TILES; ++i) {
+            mbar_init(qfull + 8 * i, 4);
+            mbar_init(odone + 8 * i, 1);
+            mbar_init(pvdone + 8 * i, 1);
+        }
+        for (int i = 0; i < T::TILES * T::BUFS; ++i) {
+            mbar_init(sfull + 8 * i, 1);
+            mbar_init(pfull + 8 * i, 4);
+        }
+        fence_mbar_init();
+    }
+    constexpr int kProducer = T::TILES * 4, kIssuer = kProducer + 1;
+    if (warp == kIssuer) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = s_tmem;
+    TcAt at;
+    if (first < line_pre) {
+        const int u = (int)(first / tp);
+        at = TcAt{-1, u / P.tcm_pre, u % P.tcm_pre, (int)(first % tp), tp};
+    } else {
+        const int tiles = tc_tiles(P, seq);
+        const long long in = first - line_pre - (long long)off * per_seq;
+        const int u = (int)(in / tiles);
+        at = TcAt{seq, u / P.tcm_own, u % P.tcm_own, (int)(in % tiles), tiles};
+    }
+    int left = (int)(end - first);
+
+    if (warp == kProducer) {
+        // ================================================================ copies: K and V of a tile, D / 64 boxes each
+        if (elect_one()) {
+            RingAt<T::SLOTS> r;
+            for (; left > 0 && !*fail; tc_next(P, at)) {
+                const int n = min(left, at.tiles - at.tile), s = at.seq < 0 ? 0 : at.seq;
+                const CUtensorMap *mk = at.seq < 0 ? &pre_k : &own_k, *mv = at.seq < 0 ? &pre_v : &own_v;
+                for (int j = 0; j < n && !*fail; ++j)
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        um_spin(empty + 8 * r.i, r.ph ^ 1u, fail);
+                        if (*fail) break;
+                        mbar_expect_tx(full + 8 * r.i, T::TILE_BYTES);
+#pragma unroll
+                        for (int b = 0; b < DB; ++b)
+                            tma_load_4d(ring_s + r.i * T::TILE_BYTES + b * (N * 128), v ? mv : mk, b * 64, (at.tile + j) * N, at.kvh, s,
+                                        full + 8 * r.i);
+                        r.skip(1);
+                    }
+                left -= n;
+            }
+        }
+    } else if (warp == kIssuer) {
+        // ================================================================ matrix instructions
+        if (elect_one()) {
+            constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
+            constexpr uint32_t kIdescS = (1u << 4) | kType | ((uint32_t)(N >> 3) << 17) | (8u << 24);
+            constexpr uint32_t kIdescO = (1u << 4) | kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);  // V: dims contiguous
+            RingAt<T::SLOTS> seg;  // the ring place of the segment's first K
+            uint32_t qph = 0, pph[T::TILES][T::BUFS] = {};
+            for (; left > 0 && !*fail; tc_next(P, at)) {
+                const int n = min(left, at.tiles - at.tile);
+                const int two = T::TILES == 2 && (at.seq < 0 ? P.tc2_pre : P.tc2_own);
+                // tile i of row tile w is key tile `i` of the segment, or 2 i + w when they take turns
+                auto count = [&](int w) { return two ? (n + 1 - w) >> 1 : n; };
+                auto place = [&](int w, int i, int v) {
+                    RingAt<T::SLOTS> r = seg;
+                    r.skip(2 * (two ? 2 * i + w : i) + v);
+                    return r;
+                };
+                auto scores = [&](int w, int i) {
+                    const RingAt<T::SLOTS> r = place(w, i, 0);
+                    if (i == 0) um_spin(qfull + 8 * w, (qph >> w) & 1u, fail);
+                    if (w == 0 || two) um_spin(full + 8 * r.i, r.ph, fail);
+                    tmem_fence_after();
+                    const uint32_t d = tmem + (w * T::BUFS + i % T::BUFS) * 128 + T::S_COL;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        umma_f16_ss(d, desc_sw128(q_s + w * T::Q_BYTES + (k >> 2) * (128 * 128), 16) + (k & 3) * 2,
+                                    desc_sw128(ring_s + r.i * T::TILE_BYTES + (k >> 2) * (N * 128), 16) + (k & 3) * 2, kIdescS, k > 0);
+                    if (w == T::TILES - 1 || two) umma_commit(empty + 8 * r.i);
+                    umma_commit(sfull + 8 * (w * T::BUFS + i % T::BUFS));
+                };
+                int most = 0;
+                for (int b = 0; b < T::BUFS; ++b)
+                    for (int w = 0; w < T::TILES; ++w)
+                        if (b < count(w)) scores(w, b);
+                for (int w = 0; w < T::TILES; ++w) {
+                    most = max(most, count(w));
+                    if (count(w)) qph ^= 1u << w;
+                }
+                for (int i = 0; i < most && !*fail; ++i)
+#pragma unroll
+                    for (int w = 0; w < T::TILES; ++w) {
+                        if (i >= count(w)) continue;
+                        const RingAt<T::SLOTS> r = place(w, i, 1);
+                        const int buf = w * T::BUFS + i % T::BUFS;
+                        um_spin(pfull + 8 * buf, pph[w][i % T::BUFS], fail);
+                        pph[w][i % T::BUFS] ^= 1u;
+                        if (w == 0 || two) um_spin(full + 8 * r.i, r.ph, fail);
+                        tmem_fence_after();
+#pragma unroll
+                        for (int k = 0; k < N / 16; ++k)
+#pragma unroll
+                            for (int t = 0; t < T::TERMS; ++t)
+                                umma_f16_ts(tmem + T::O_COL + w * D, tmem + buf * 128 + (k >> 1) * (16 * T::TERMS) + t * 16 + (k & 1) * 8,
+                                            desc_sw128(ring_s + r.i * T::TILE_BYTES + k * 2048, N * 128), kIdescO, i > 0 || k > 0 || t > 0);
+                        if (w == T::TILES - 1 || two) umma_commit(empty + 8 * r.i);
+                        if (T::BUFS > 1) umma_commit(pvdone + 8 * w);
+                        if (i + 1 == count(w))
+                            umma_commit(odone + 8 * w);
+                        else if (i + T::BUFS < count(w))
+                            scores(w, i + T::BUFS);
+                    }
+                seg.skip(2 * n % T::SLOTS);
+                if ((2 * n / T::SLOTS) & 1) seg.ph ^= 1u;
+                left -= n;
+            }
+        }
+    } else {
+        // ================================================================ softmax: one row of row tile w per thread
+        const int w = warp >> 2, lane = tid & 31, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
+        const uint32_t flip = P.scale2 < 0.0f ? 0x80008000u : 0u;  // the sign of the scale goes into Q: scores only need a positive one
+        const float scale = fabsf(P.scale2);
+        uint32_t sph[T::BUFS] = {}, oph = 0, pvph = 1;  // pvph: parity of the product before this tile's
+        for (; left > 0; tc_next(P, at)) {
+            const int n = min(left, at.tiles - at.tile);
+            const int two = T::TILES == 2 && (at.seq < 0 ? P.tc2_pre : P.tc2_own);
+            const int mine = two ? (n + 1 - w) >> 1 : n;
+            const int M = (at.seq < 0 ? P.S : P.rows) * P.G, row0 = at.seq < 0 ? 0 : at.seq * P.rows;
+            const int r = two ? at.mt * 128 + row : at.mt * T::ROWS + w * 128 + row;
+            float m = -INFINITY, l = 0.0f;
+            if (mine) {
+                const uint16_t *src = P.q + ((long long)(row0 + r / P.G) * P.H + at.kvh * P.G + r % P.G) * D;
+                uint8_t *to = base + w * T::Q_BYTES + row * 128;
+#pragma unroll 4
+                for (int ch = 0; ch < D / 8; ++ch) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (r < M) {
+                        v = *reinterpret_cast<const uint4 *>(src + ch * 8);
+                        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+                    }
+                    *reinterpret_cast<uint4 *>(to + (ch >> 3) * (128 * 128) + (((ch & 7) ^ (row & 7)) << 4)) = v;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                mbar_arrive_lane0(qfull + 8 * w, lane);
+            }
+            for (int i = 0; i < mine; ++i) {
+                const int bi = i % T::BUFS, buf = w * T::BUFS + bi;
+                const uint32_t region = tmem + lanes + buf * 128;
+                um_spin(sfull + 8 * buf, sph[bi], fail);
+                sph[bi] ^= 1u;
+                tmem_fence_after();
+                float s[N];
+#pragma unroll
+                for (int q = 0; q < N / 32; ++q) tmem_ld32(region + T::S_COL + q * 32, s + q * 32);
+#pragma unroll
+                for (int q = 0; q < N / 32; ++q) tmem_wait_ld32(s + q * 32);
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int e = 4; e < N; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                if (i == 0) {
+                    m = top;
+                } else if (__any_sync(0xffffffffu, top > m + 4.0f)) {
+                    // O of this row tile is at rest: the product before was committed with these scores, or is waited for
+                    if (T::BUFS > 1) {
+                        um_spin(pvdone + 8 * w, pvph, fail);
+                        tmem_fence_after();
+                    }
+                    const float to = top > m + 4.0f ? top : m;
+                    const float f = to == m ? 1.0f : ex2(m - to);
+                    m = to;
+                    l *= f;
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 32) {
+                        float o[32];
+                        tmem_ld32(tmem + lanes + T::O_COL + w * D + d, o);
+                        tmem_wait_ld32(o);
+                        uint32_t u[16];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[h * 16 + e] * f);
+                            tmem_st16(tmem + lanes + T::O_COL + w * D + d + h * 16, u);
+                        }
+                    }
+                }
+                pvph ^= 1u;
+                if (P.scores && at.seq >= 0 && r < M) {
+                    float *x = P.scores + (((long long)at.seq * nkv + at.kvh) * M + r) * P.own.cap +
+                               (long long)(at.tile + (two ? 2 * i + w : i)) * N;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) x[e] = s[e] * scale;
+                }
+                const float ms = (m == -INFINITY ? 0.0f : m) - kAtLift<BF16>;
+                float sum[4] = {};
+#pragma unroll
+                for (int q = 0; q < N / 32; ++q) {
+                    float *x = s + q * 32;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        x[e] = ex2(fmaf(x[e], scale, -ms));
+                        sum[e & 3] += x[e];
+                    }
+#pragma unroll
+                    for (int t = 0; t < T::TERMS; ++t) {
+                        uint32_t u[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            u[e] = pack16<BF16>(x[2 * e], x[2 * e + 1]);
+                            if (t + 1 < T::TERMS) {
+                                x[2 * e] -= low16<BF16>(u[e]);
+                                x[2 * e + 1] -= high16<BF16>(u[e]);
+                            }
+                        }
+                        tmem_st16(region + q * (16 * T::TERMS) + t * 16, u);
+                    }
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tmem_fence_before();
+                __syncwarp();
+                mbar_arrive_lane0(pfull + 8 * buf, lane);
+            }
+            // the segment's partial result
+            const int unit = at.seq < 0 ? at.kvh * P.tcm_pre + at.mt
+                                        : nkv * P.tcm_pre + (at.seq * nkv + at.kvh) * P.tcm_own + at.mt;
+            const long long to = ((long long)unit + c) * T::ROWS + w * 128 + row;
+            if (mine) {
+                um_spin(odone + 8 * w, oph, fail);
+                oph ^= 1u;
+                tmem_fence_after();
+            }
+            if (r < M) P.tc_ml[to] = make_float2(m, l);
+#pragma unroll 1
+            for (int d = 0; d < D; d += 32) {
+                float o[32];
+                if (mine) {
+                    tmem_ld32(tmem + lanes + T::O_COL + w * D + d, o);
+                    tmem_wait_ld32(o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                }
+                if (r < M)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4 *>(P.tc_part + to * D + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+            tmem_fence_before();
+            left -= n;
+        }
+    }
+    __syncwarp();
+    tmem_fence_before();
+    __syncthreads();
+    if (tid == 0 && *fail) {
+        report_error(P.err, kErrBarrierTimeout);
+        const long long t0 = clock64();  // copies that are under way land before the shared memory is given back
+        while (clock64() - t0 < 4000000LL) {
+        }
+    }
+    __syncthreads();
+    if (warp == kIssuer) {
+        tmem_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+}  // namespace pgb
