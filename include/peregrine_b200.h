@@ -243,8 +243,8 @@ int coli_cuda_pipe_argmax(int device, int *ids_dev, const float *logits_dev, int
  * is left as it was.  A refused call prints the reason, launches nothing and returns 0.
  *
  * ColiCudaKv names one layer's cache of keys and values: element (sequence, kv head, slot, d) of k and v is at
- * sequence * seq_stride + head * head_stride + slot * slot_stride + d (strides in elements, multiples of 8;
- * all three 0: dense [n_seq, n_kv, cap, D]); k and v 16-byte aligned, 1 <= n_kv, 1 <= n_seq, 1 <= cap, D one of
+ * sequence * seq_stride + head * head_stride + slot * slot_stride + d (strides in elements, multiples of 8
+ * below 2^39; all three 0: dense [n_seq, n_kv, cap, D]); k and v 16-byte aligned, 1 <= n_kv, 1 <= n_seq, 1 <= cap, D one of
  * 64, 128, 256; dtype 1 = bf16, 2 = f16.  pos and acc are dense [n_seq, n_kv, cap] or NULL: the position each
  * slot was stored with, and the attention weight it has received so far.  Slots that were never stored may hold
  * anything: no result depends on them. */

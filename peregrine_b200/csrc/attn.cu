@@ -49,9 +49,8 @@ int kv_args(KvArgs *a, const ColiCudaKv *kv, const char *what) {
         a->head_stride = (long long)kv->cap * kv->D;
         a->seq_stride = (long long)kv->n_kv * a->head_stride;
     }
-    const long long limit = 1ll << 44;  // offsets stay far from 64-bit overflow
-    for (const long long s : {a->seq_stride, a->head_stride, a->slot_stride})
-        if (s < 0 || s > limit || (s & 7)) return refuse("%s: cache strides must be multiples of 8", what);
+    for (const long long s : {a->seq_stride, a->head_stride, a->slot_stride})  // the copy engine's strides end at 2^40 bytes
+        if (s < 0 || s >= 1ll << 39 || (s & 7)) return refuse("%s: cache strides must be multiples of 8", what);
     if (a->slot_stride < kv->D || (kv->n_kv > 1 && a->head_stride < kv->D) || (kv->n_seq > 1 && a->seq_stride < kv->D))
         return refuse("%s: cache strides overlap", what);
     return 1;
@@ -90,27 +89,30 @@ struct NormRopeLaunch {
     }
 };
 
-int row_tile(long long m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
-
-// CTAs of the split kernel: as many as are resident at once (shared memory of a CTA: 73, 113 or 193 kB).
-int attn_ctas(int D, int sms) { return sms * (D == 64 ? 3 : D == 128 ? 2 : 1); }
-
 // Problems with more row vectors than this go to the tensor-memory kernel, whose tiles have 128 rows.
-constexpr int kTcRows = 32;
+constexpr int kTcRows = 16;
+
+// Row tile of the split kernel.
+int row_tile(int rows, int H, int n_kv) { return rows * (H / n_kv) <= 8 ? 8 : 16; }
+// Its CTAs: as many as are resident at once.
+int attn_ctas(int D, int rt, int sms) {
+    if (D == 64) return sms * (rt == 8 ? SplitShape<64, 8>::PER_SM : SplitShape<64, 16>::PER_SM);
+    if (D == 128) return sms * (rt == 8 ? SplitShape<128, 8>::PER_SM : SplitShape<128, 16>::PER_SM);
+    return sms * (rt == 8 ? SplitShape<256, 8>::PER_SM : SplitShape<256, 16>::PER_SM);
+}
 
 // Shapes and the scratch's layout from the description of a call; bytes needed, or 0 for numbers past the kernels' range.
 size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, int rows, bool wide_weights, int sms, char *work) {
     const long long m_own = (long long)rows * (H / own.n_kv), m_pre = (long long)S * (H / own.n_kv);
     P->G = H / own.n_kv;
-    P->rt_own = row_tile(m_own);
-    P->rt_pre = row_tile(m_pre);
-    P->rt_max = prefix_len ? (P->rt_pre > P->rt_own ? P->rt_pre : P->rt_own) : P->rt_own;
-    const long long mt_own = (m_own + P->rt_own - 1) / P->rt_own, mt_pre = prefix_len ? (m_pre + P->rt_pre - 1) / P->rt_pre : 0;
+    const int rt = row_tile(rows, H, own.n_kv);
+    const long long mt_own = (m_own + rt - 1) / rt, mt_pre = prefix_len ? (m_pre + rt - 1) / rt : 0;
     const long long units = own.n_kv * (mt_pre + own.n_seq * mt_own);
-    if (units > 0x3fffffff || m_pre > 0x3fffffff) return 0;
+    // tiles of 64 keys of a line are counted in 32 bits per sequence
+    if (units > 0x3fffffff || m_pre > 0x3fffffff || ((long long)own.cap / 64 + 1) * own.n_kv * mt_own > 0x3fffffff) return 0;
     P->mt_own = (int)mt_own;
     P->mt_pre = (int)mt_pre;
-    P->ctas = attn_ctas(own.D, sms);
+    P->ctas = attn_ctas(own.D, rt, sms);
     P->tc_keys = own.D == 256 || wide_weights ? 64 : 128;
     P->tc_rows = own.D == 256 ? 128 : 256;
     P->tc_ctas = sms;
@@ -127,22 +129,20 @@ size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, i
         at += (bytes + 255) & ~(size_t)255;
         return p;
     };
-    const size_t rows_all = (size_t)(units + P->ctas) * P->rt_max;
-    P->part = reinterpret_cast<float *>(take(rows_all * own.D * 4));
-    P->ml = reinterpret_cast<float2 *>(take(rows_all * 8));
-    P->offs = reinterpret_cast<int *>(take(((size_t)own.n_seq + 1) * 4));
+    const bool tc = P->tc_pre || P->tc_own;
+    const size_t tc_units = tc ? own.n_kv * (P->tcm_pre + (size_t)own.n_seq * P->tcm_own) : 0;
+    const size_t split_rows = ((size_t)units + P->ctas) * rt, tc_rows = tc ? (tc_units + P->tc_ctas) * P->tc_rows : 0;
+    P->tc_row0 = (long long)split_rows;
+    P->part = reinterpret_cast<float *>(take((split_rows + tc_rows) * own.D * 4));
+    P->ml = reinterpret_cast<float2 *>(take((split_rows + tc_rows) * 8));
+    P->cta_of = reinterpret_cast<int2 *>(take((size_t)units * 8));
+    P->tc_cta_of = reinterpret_cast<int2 *>(take(tc_units * 8));
     P->scores = own.acc ? reinterpret_cast<float *>(take((size_t)own.n_seq * own.n_kv * m_own * own.cap * 4)) : nullptr;
-    if (P->tc_pre || P->tc_own) {
-        const size_t tc_all = ((size_t)own.n_kv * (P->tcm_pre + (size_t)own.n_seq * P->tcm_own) + P->tc_ctas) * P->tc_rows;
-        P->tc_part = reinterpret_cast<float *>(take(tc_all * own.D * 4));
-        P->tc_ml = reinterpret_cast<float2 *>(take(tc_all * 8));
-        P->tc_offs = reinterpret_cast<int *>(take(((size_t)own.n_seq + 1) * 4));
-    }
     return at;
 }
 
 // Copies of [keys][64 dims] boxes of a cache, swizzled by 128 bytes.
-int kv_map(CUtensorMap *m, const void *p, const KvArgs &kv, int dtype, int keys) {
+int kv_map(CUtensorMap *m, const void *p, const KvArgs &kv, int dtype) {
     typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -160,7 +160,7 @@ int kv_map(CUtensorMap *m, const void *p, const KvArgs &kv, int dtype, int keys)
     const long long head = kv.n_kv > 1 ? kv.head_stride : kv.slot_stride, seq = kv.n_seq > 1 ? kv.seq_stride : kv.slot_stride;
     const cuuint64_t dims[4] = {(cuuint64_t)kv.D, (cuuint64_t)kv.cap, (cuuint64_t)kv.n_kv, (cuuint64_t)kv.n_seq};
     const cuuint64_t strides[3] = {(cuuint64_t)kv.slot_stride * 2, (cuuint64_t)head * 2, (cuuint64_t)seq * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)keys, 1, 1}, es[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, kAtKeys, 1, 1}, es[4] = {1, 1, 1, 1};
     return enc(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(p), dims, strides,
                box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -193,10 +193,11 @@ struct AttnLaunch {
     const AttnArgs &P;
     const CUtensorMap *maps;  // of the prefix's and the own keys and values
     cudaStream_t stream;
-    template <int D, bool BF16, bool F32>
+    template <int D, bool BF16, bool F32, int RT>
     int run() const {
-        auto split = attn_split_kernel<D, BF16, F32>;
-        if (!opt_in(split, kAtSmem<D>)) return 0;
+        constexpr int kSmem = SplitShape<D, RT>::SMEM;
+        auto split = attn_split_kernel<D, BF16, F32, RT>;
+        if (!opt_in(split, kSmem)) return 0;
         if (P.tc_pre || P.tc_own) {
             using T = TcShape<D, BF16, F32>;
             static_assert(T::ROWS == (D == 256 ? 128 : 256) && T::N == (D == 256 || (BF16 && F32) ? 64 : 128), "as planned");
@@ -205,19 +206,20 @@ struct AttnLaunch {
             tc<<<dim3(P.tc_ctas), T::THREADS, T::SMEM, stream>>>(P, maps[0], maps[1], maps[2], maps[3]);
             if (!launched("attention tensor launch")) return 0;
             // needs nothing of the one before: it fills the SMs that this leaves, and ends after it
-            if (!launch_early(split, P.ctas, kAtThreads, kAtSmem<D>, stream, "attention launch", P)) return 0;
+            if (!launch_early(split, P.ctas, kAtThreads, kSmem, stream, "attention launch", P, maps[0], maps[1], maps[2], maps[3])) return 0;
         } else {
-            split<<<dim3(P.ctas), kAtThreads, kAtSmem<D>, stream>>>(P);
+            split<<<dim3(P.ctas), kAtThreads, kSmem, stream>>>(P, maps[0], maps[1], maps[2], maps[3]);
             if (!launched("attention launch")) return 0;
         }
         // waits on the device for the end of the launches before
         const int chunks = P.own.acc ? (P.own.cap + 2 * kAtCombine - 1) / (2 * kAtCombine) : 0;
         const unsigned grid = (unsigned)((long long)P.S * P.H + (long long)chunks * P.own.n_seq * P.own.n_kv);
-        return launch_early(attn_join_kernel<D, BF16>, grid, kAtCombine, 0, stream, "attention join launch", P, chunks);
+        return launch_early(attn_join_kernel<D, BF16>, grid, kAtCombine, 0, stream, "attention join launch", P, RT, chunks);
     }
     template <int D, bool BF16>
     int operator()() const {
-        return P.out_f32 ? run<D, BF16, true>() : run<D, BF16, false>();
+        if (row_tile(P.rows, P.H, P.own.n_kv) == 8) return P.out_f32 ? run<D, BF16, true, 8>() : run<D, BF16, false, 8>();
+        return P.out_f32 ? run<D, BF16, true, 16>() : run<D, BF16, false, 16>();
     }
 };
 
@@ -314,9 +316,14 @@ PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, 
     DeviceGuard g(c.device);
     if (!g.ok()) return refuse("%s: device %d cannot be selected", what, device);
     CUtensorMap maps[4] = {};
-    if ((P.tc_pre && !(kv_map(&maps[0], P.pre.k, P.pre, own->dtype, P.tc_keys) && kv_map(&maps[1], P.pre.v, P.pre, own->dtype, P.tc_keys))) ||
-        (P.tc_own && !(kv_map(&maps[2], P.own.k, P.own, own->dtype, P.tc_keys) && kv_map(&maps[3], P.own.v, P.own, own->dtype, P.tc_keys))))
-        return refuse("%s: the cache's strides cannot be described to the copy engine", what);
+    const int type = own->dtype;
+    if ((prefix_len && !(kv_map(&maps[0], P.pre.k, P.pre, type) && kv_map(&maps[1], P.pre.v, P.pre, type))) ||
+        !(kv_map(&maps[2], P.own.k, P.own, type) && kv_map(&maps[3], P.own.v, P.own, type)))
+        return refuse("%s: the cache cannot be described to the copy engine", what);
+    if (!prefix_len) {  // not used
+        maps[0] = maps[2];
+        maps[1] = maps[3];
+    }
     return by_type(own->D, own->dtype, AttnLaunch{P, maps, c.stream});
 }
 

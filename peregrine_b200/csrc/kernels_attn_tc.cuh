@@ -88,8 +88,8 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     const long long line_pre = (long long)nkv * P.tcm_pre * tp;
     long long first, end;
     int seq = 0, off = 0;
-    if (!line_share<T::THREADS / 32>(P.own.n_seq, [&](int b) { return tc_tiles(P, b); }, per_seq, line_pre, P.tc_ctas, P.tc_offs, first,
-                                     end, seq, off))
+    if (!line_share<T::THREADS / 32>(P.own.n_seq, [&](int b) { return tc_tiles(P, b); }, per_seq, line_pre, P.tc_ctas, first, end, seq,
+                                     off))
         return;
     uint8_t *base = tc_smem_raw + ((1024 - (smem_u32(tc_smem_raw) & 1023)) & 1023);
     const uint32_t q_s = smem_u32(base), ring_s = q_s + T::TILES * T::Q_BYTES;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     int left = (int)(end - first);
 
     if (warp == kProducer) {
-        // ================================================================ copies: K and V of a tile, D / 64 boxes each
+        // ================================================================ copies: K and V of a tile in boxes of 64 keys x 64 dims
         if (elect_one()) {
             RingAt<T::SLOTS> r;
             for (; left > 0 && !*fail; tc_next(P, at)) {
@@ -146,8 +146,10 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                         mbar_expect_tx(full + 8 * r.i, T::TILE_BYTES);
 #pragma unroll
                         for (int b = 0; b < DB; ++b)
-                            tma_load_4d(ring_s + r.i * T::TILE_BYTES + b * (N * 128), v ? mv : mk, b * 64, (at.tile + j) * N, at.kvh, s,
-                                        full + 8 * r.i);
+#pragma unroll
+                            for (int h = 0; h < N / 64; ++h)
+                                tma_load_4d(ring_s + r.i * T::TILE_BYTES + b * (N * 128) + h * 8192, v ? mv : mk, b * 64,
+                                            (at.tile + j) * N + h * 64, at.kvh, s, full + 8 * r.i);
                         r.skip(1);
                     }
                 left -= n;
@@ -237,14 +239,19 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             if (mine) {
                 const uint16_t *src = P.q + ((long long)(row0 + r / P.G) * P.H + at.kvh * P.G + r % P.G) * D;
                 uint8_t *to = base + w * T::Q_BYTES + row * 128;
-#pragma unroll 4
-                for (int ch = 0; ch < D / 8; ++ch) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (r < M) {
-                        v = *reinterpret_cast<const uint4 *>(src + ch * 8);
-                        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+#pragma unroll
+                for (int c0 = 0; c0 < D / 8; c0 += 16) {
+                    constexpr int B = D / 8 < 16 ? D / 8 : 16;  // loads under way together
+                    uint4 v[B];
+#pragma unroll
+                    for (int e = 0; e < B; ++e)
+                        v[e] = r < M ? *reinterpret_cast<const uint4 *>(src + (c0 + e) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < B; ++e) {
+                        const int ch = c0 + e;
+                        v[e].x ^= flip, v[e].y ^= flip, v[e].z ^= flip, v[e].w ^= flip;
+                        *reinterpret_cast<uint4 *>(to + (ch >> 3) * (128 * 128) + (((ch & 7) ^ (row & 7)) << 4)) = v[e];
                     }
-                    *reinterpret_cast<uint4 *>(to + (ch >> 3) * (128 * 128) + (((ch & 7) ^ (row & 7)) << 4)) = v;
                 }
                 fence_proxy_async();
                 __syncwarp();
@@ -331,13 +338,15 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             // the segment's partial result
             const int unit = at.seq < 0 ? at.kvh * P.tcm_pre + at.mt
                                         : nkv * P.tcm_pre + (at.seq * nkv + at.kvh) * P.tcm_own + at.mt;
-            const long long to = ((long long)unit + c) * T::ROWS + w * 128 + row;
+            const long long to = P.tc_row0 + ((long long)unit + c) * T::ROWS + w * 128 + row;
+            if (tid == 0 && at.tile == 0) P.tc_cta_of[unit].x = c;
+            if (tid == 0 && at.tile + n == at.tiles) P.tc_cta_of[unit].y = c;
             if (mine) {
                 um_spin(odone + 8 * w, oph, fail);
                 oph ^= 1u;
                 tmem_fence_after();
             }
-            if (r < M) P.tc_ml[to] = make_float2(m, l);
+            if (r < M) P.ml[to] = make_float2(m, l);
 #pragma unroll 1
             for (int d = 0; d < D; d += 32) {
                 float o[32];
@@ -351,7 +360,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                 if (r < M)
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4 *>(P.tc_part + to * D + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        *reinterpret_cast<float4 *>(P.part + to * D + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
             tmem_fence_before();
             left -= n;
