@@ -212,9 +212,12 @@ struct AttnLaunch {
             if (!launched("attention launch")) return 0;
         }
         // waits on the device for the end of the launches before
-        const int chunks = P.own.acc ? (P.own.cap + 2 * kAtCombine - 1) / (2 * kAtCombine) : 0;
-        const unsigned grid = (unsigned)((long long)P.S * P.H + (long long)chunks * P.own.n_seq * P.own.n_kv);
-        return launch_early(attn_join_kernel<D, BF16>, grid, kAtCombine, 0, stream, "attention join launch", P, RT, chunks);
+        const long long vectors = (long long)P.S * P.H, chunks = P.own.acc ? (P.own.cap + kAtChunk - 1) / kAtChunk : 0;
+        const bool few = vectors < 4 * P.tc_ctas;
+        const int row_ctas = (int)(few ? vectors : (vectors + 3) / 4);
+        const unsigned grid = (unsigned)(row_ctas + chunks * P.own.n_seq * P.own.n_kv);
+        return launch_early(few ? attn_join_kernel<D, BF16, 4> : attn_join_kernel<D, BF16, 1>, grid, kAtCombine, 0, stream,
+                            "attention join launch", P, RT, row_ctas, (int)chunks);
     }
     template <int D, bool BF16>
     int operator()() const {
@@ -284,7 +287,7 @@ PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, 
     if (!kv_args(&P.own, own, what) || !rows_ok(S, H, P.own, rows_per_seq, what)) return 0;
     if (rows_per_seq > 64) return refuse("%s: %d rows of a sequence are more than 64", what, rows_per_seq);
     if (H % own->n_kv) return refuse("%s: %d heads are no multiple of %d", what, H, own->n_kv);
-    if ((long long)S * H + (own->acc ? (long long)(own->cap / 256 + 1) * own->n_seq * own->n_kv : 0) > 0x7fffffffll)
+    if ((long long)S * H + (own->acc ? (long long)(own->cap / kAtChunk + 1) * own->n_seq * own->n_kv : 0) > 0x7fffffffll)
         return refuse("%s: too many rows and heads", what);
     if (!out_dev || !q_dev || !base_dev || !work_dev) return refuse("%s: null pointer", what);
     if (!aligned(out_dev, 16) || !aligned(q_dev, 16) || !aligned(base_dev, 4) || !aligned(mask_dev, 8) || !aligned(work_dev, 256))

@@ -22,6 +22,7 @@ namespace pgb {
 constexpr int kAtKeys = 64;      // keys of a tile
 constexpr int kAtThreads = 160;  // 4 warps with 16 keys of a tile each, one that issues the copies
 constexpr int kAtCombine = 128;
+constexpr int kAtChunk = 1024;  // slots whose weights one CTA adds up
 
 struct AttnArgs {
     void *out;
@@ -614,148 +615,185 @@ __global__ void __launch_bounds__(kAtThreads, SplitShape<D, RT>::PER_SM)
     griddep_wait();  // the joining launch waits for this one alone, and needs the tensor-memory kernel's results too
 }
 
-// Up to six runs of partials of a row vector: `n` rows of part / ml from row `at` on, `stride` rows apart.
-struct AttnList {
-    long long at[6];
-    int stride[6], n[6], total;
+// The partials of a row vector lie in up to six runs of rows of part / ml: `n` rows, `stride` apart, from row `at` on.
+struct AttnRun {
+    long long at;
+    int stride, n;
 };
 // Run j of row vector r (within its sequence) of a (sequence, kv head): the prefix's and the own slots' from the split kernel (0, 1),
 // the same from the tensor-memory kernel, each in up to two halves (2 to 5).
-__device__ __forceinline__ void attn_list(const AttnArgs &P, AttnList &L, int j, int seq, int kvh, int r, int rt) {
+__device__ __forceinline__ AttnRun attn_run(const AttnArgs &P, int j, int seq, int kvh, int r, int rt) {
     const int nkv = P.own.n_kv, rp = seq * P.rows * P.G + r;
     const bool own = j == 1 || j >= 4, tc = j >= 2;
     const int q = own ? r : rp;
     bool there;
-    int unit, row;
+    int unit, row, t = rt;
     if (!tc) {
         const int mt = own ? P.mt_own : P.mt_pre;
         there = own ? own_tiles(P, seq) > 0 : P.mt_pre && P.prefix_len > P.cut_pre;
-        unit = (own ? nkv * P.mt_pre + seq * nkv * P.mt_own : 0) + kvh * mt + q / rt;
-        row = q % rt;
+        unit = (own ? nkv * P.mt_pre + seq * nkv * P.mt_own : 0) + kvh * mt + q / t;
+        row = q % t;
     } else {
-        const int two = own ? P.tc2_own : P.tc2_pre, t = two ? 128 : P.tc_rows;
+        const int two = own ? P.tc2_own : P.tc2_pre;
+        t = two ? 128 : P.tc_rows;
         there = (own ? P.tc_own && own_cut(P, seq) > 0 : P.tc_pre) && (two || !(j & 1));
         unit = (own ? nkv * P.tcm_pre + seq * nkv * P.tcm_own + kvh * P.tcm_own : kvh * P.tcm_pre) + q / t;
         row = q % t + (j & 1) * 128;
-        rt = P.tc_rows;
+        t = P.tc_rows;
     }
-    int n = 0;
+    AttnRun R{0, t, 0};
     if (there) {
         const int2 ends = (tc ? P.tc_cta_of : P.cta_of)[unit];
-        n = ends.y - ends.x + 1;
-        L.at[j] = ((long long)unit + ends.x) * rt + row + (tc ? P.tc_row0 : 0);
+        R.n = ends.y - ends.x + 1;
+        R.at = ((long long)unit + ends.x) * t + row + (tc ? P.tc_row0 : 0);
     }
-    L.n[j] = n;
-    L.stride[j] = rt;
+    return R;
 }
-__device__ __forceinline__ long long attn_part(const AttnList &L, int j) {
-    int k = 0;
-    while (j >= L.n[k]) j -= L.n[k++];
-    return L.at[k] + (long long)j * L.stride[k];
+// All runs in the registers of every lane, and what the partials' statistics say: maximum and sum over all of them.
+struct AttnRow {
+    AttnRun run[6];
+    int n;
+    float m, l;
+    __device__ __forceinline__ long long at(int j) const {
+        long long r = 0;
+#pragma unroll
+        for (int k = 0; k < 6; ++k) {
+            if (j >= 0 && j < run[k].n) r = run[k].at + (long long)j * run[k].stride;
+            j -= run[k].n;
+        }
+        return r;
+    }
+};
+__device__ __forceinline__ void attn_row(const AttnArgs &P, AttnRow &R, int lane, int seq, int kvh, int r, int rt) {
+    const AttnRun mine = attn_run(P, min(lane, 5), seq, kvh, r, rt);
+    R.n = 0;
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+        R.run[k].at = __shfl_sync(0xffffffffu, mine.at, k);
+        R.run[k].stride = __shfl_sync(0xffffffffu, mine.stride, k);
+        R.run[k].n = __shfl_sync(0xffffffffu, mine.n, k);
+        R.n += R.run[k].n;
+    }
+    float m = -INFINITY, l = 0.0f;
+    for (int j = lane; j < R.n; j += 32) {
+        const float2 ml = P.ml[R.at(j)];
+        const float to = fmaxf(m, ml.x);
+        if (to != -INFINITY) {
+            l = l * ex2(m - to) + ml.y * ex2(ml.x - to);
+            m = to;
+        } else {
+            l += ml.y;  // zero, or NaN
+        }
+    }
+    float top = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top == -INFINITY) top = 0.0f;
+    l *= ex2(m - top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    R.m = top;
+    R.l = l;
 }
 
-// Joins the partials: CTAs [0, S x H) one row vector each; with acc, further CTAs 256 slots of one (sequence, kv head) each.
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P, int rt, int chunks) {
+// Joins the partials.  The first `row_ctas` CTAs take 4 / WPR row vectors each, WPR warps to one (4 where there are too few
+// row vectors to fill the device); with acc, further CTAs take 1024 slots of one (sequence, kv head) each.
+template <int D, bool BF16, int WPR>
+__global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P, int rt, int row_ctas, int chunks) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     griddep_wait();
-    if (blockIdx.x < (unsigned)(P.S * P.H)) {
+    if (blockIdx.x < (unsigned)row_ctas) {
         constexpr int E = D / 32;
-        __shared__ AttnList L;
-        __shared__ float s_m[4], s_l[4], s_o[4][D];
-        const int row = blockIdx.x / P.H, h = blockIdx.x % P.H, seq = row / P.rows, kvh = h / P.G;
+        __shared__ float s_o[WPR][WPR == 1 ? 1 : D];
+        const int u = blockIdx.x * (4 / WPR) + warp / WPR, sub = warp % WPR;
+        if (u >= P.S * P.H) return;
+        const int row = u / P.H, h = u % P.H, seq = row / P.rows, kvh = h / P.G;
         if (P.base[seq] < 0) return;
-        if (threadIdx.x < 6) attn_list(P, L, threadIdx.x, seq, kvh, (row % P.rows) * P.G + h % P.G, rt);
-        __syncthreads();
-        const int n = L.n[0] + L.n[1] + L.n[2] + L.n[3] + L.n[4] + L.n[5];
-        float m = -INFINITY;
-        for (int j = threadIdx.x; j < n; j += kAtCombine) m = fmaxf(m, P.ml[attn_part(L, j)].x);
+        AttnRow R;
+        attn_row(P, R, lane, seq, kvh, (row % P.rows) * P.G + h % P.G, rt);
+        float o[E] = {};
+        for (int j0 = 0; j0 < R.n; j0 += 32) {
+            const int j = j0 + lane;
+            const long long mine = j < R.n ? R.at(j) : 0;
+            const float w = j < R.n ? ex2(P.ml[mine].x - R.m) : 0.0f;
+            const int n = min(32, R.n - j0);
+#pragma unroll 8
+            for (int i = sub; i < n; i += WPR) {
+                const float f = __shfl_sync(0xffffffffu, w, i);
+                const float *src = P.part + __shfl_sync(0xffffffffu, mine, i) * D + lane * E;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) s_m[warp] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-        if (m == -INFINITY) m = 0.0f;
-        float o[E] = {}, l = 0.0f;
-#pragma unroll 4
-        for (int j = warp; j < n; j += 4) {
-            const long long at = attn_part(L, j);
-            const float2 ml = P.ml[at];
-            const float f = ex2(ml.x - m);
-            l = fmaf(ml.y, f, l);
-            const float *src = P.part + at * D + lane * E;
-#pragma unroll
-            for (int e = 0; e < E; e += 2) {
-                const float2 v = *reinterpret_cast<const float2 *>(src + e);
-                o[e] = fmaf(v.x, f, o[e]);
-                o[e + 1] = fmaf(v.y, f, o[e + 1]);
+                for (int e = 0; e < E; e += E < 4 ? 2 : 4)
+                    if (E < 4) {
+                        const float2 v = *reinterpret_cast<const float2 *>(src + e);
+                        o[e] = fmaf(v.x, f, o[e]);
+                        o[e + 1] = fmaf(v.y, f, o[e + 1]);
+                    } else {
+                        const float4 v = *reinterpret_cast<const float4 *>(src + e);
+                        o[e] = fmaf(v.x, f, o[e]);
+                        o[e + 1] = fmaf(v.y, f, o[e + 1]);
+                        o[(e + 2) % E] = fmaf(v.z, f, o[(e + 2) % E]);
+                        o[(e + 3) % E] = fmaf(v.w, f, o[(e + 3) % E]);
+                    }
             }
         }
+        if (WPR > 1) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-        if (lane == 0) s_l[warp] = l;
-        __syncthreads();
-        l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const long long to = (long long)blockIdx.x * D;
-        for (int d = threadIdx.x * 2; d < D; d += kAtCombine * 2) {
-            const float x = ((s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d])) * inv;
-            const float y = ((s_o[0][d + 1] + s_o[1][d + 1]) + (s_o[2][d + 1] + s_o[3][d + 1])) * inv;
-            if (P.out_f32)
-                *reinterpret_cast<float2 *>(static_cast<float *>(P.out) + to + d) = make_float2(x, y);
-            else
-                *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(P.out) + to + d) = pack16<BF16>(x, y);
+            for (int e = 0; e < E; ++e) s_o[sub][WPR == 1 ? 0 : lane * E + e] = o[e];
+            __syncthreads();
+            if (sub) return;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int d = WPR == 1 ? 0 : lane * E + e;
+                o[e] = (s_o[0][d] + s_o[1 % WPR][d]) + (s_o[2 % WPR][d] + s_o[3 % WPR][d]);
+            }
+        }
+        const float inv = R.l == 0.0f ? 0.0f : 1.0f / R.l;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= inv;
+        const long long to = (long long)u * D + lane * E;
+        if (P.out_f32) {
+#pragma unroll
+            for (int e = 0; e < E; e += 2) *reinterpret_cast<float2 *>(static_cast<float *>(P.out) + to + e) = make_float2(o[e], o[e + 1]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; e += 2)
+                *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(P.out) + to + e) = pack16<BF16>(o[e], o[e + 1]);
         }
         return;
     }
     // acc[slot] += sum over the group's row vectors of 2^(x - m) / l
-    const int u = blockIdx.x - P.S * P.H, g = u / chunks, chunk = u % chunks;
+    const int u = blockIdx.x - row_ctas, g = u / chunks, chunk = u % chunks;
     const int seq = g / P.own.n_kv, kvh = g % P.own.n_kv;
     const int keys = own_keys(P, seq);
-    const int t0 = chunk * 2 * kAtCombine;
-    if (t0 >= keys) return;
-    __shared__ AttnList lists[4];
+    const int t0 = chunk * kAtChunk + threadIdx.x;
+    if (chunk * kAtChunk >= keys) return;
+    constexpr int C = kAtChunk / kAtCombine;
     __shared__ float2 s_row[64];  // m and 1 / l of the row vectors
     const int M = P.rows * P.G;
-    float sum[2] = {0.0f, 0.0f};
+    float sum[C] = {};
     for (int r0 = 0; r0 < M; r0 += 64) {
-        __syncthreads();
+        if (r0) __syncthreads();
         for (int r = r0 + warp; r < min(M, r0 + 64); r += 4) {
-            AttnList &L = lists[warp];
-            __syncwarp();
-            if (lane < 6) attn_list(P, L, lane, seq, kvh, r, rt);
-            __syncwarp();
-            const int n = L.n[0] + L.n[1] + L.n[2] + L.n[3] + L.n[4] + L.n[5];
-            float m = -INFINITY, l = 0.0f;
-            for (int j = lane; j < n; j += 32) m = fmaxf(m, P.ml[attn_part(L, j)].x);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if (m == -INFINITY) m = 0.0f;
-            for (int j = lane; j < n; j += 32) {
-                const float2 ml = P.ml[attn_part(L, j)];
-                l = fmaf(ml.y, ex2(ml.x - m), l);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (lane == 0) s_row[r - r0] = make_float2(m - kAtLift<BF16>, l == 0.0f ? 0.0f : 1.0f / l);
+            AttnRow R;
+            attn_row(P, R, lane, seq, kvh, r, rt);
+            if (lane == 0) s_row[r - r0] = make_float2(R.m - kAtLift<BF16>, R.l == 0.0f ? 0.0f : 1.0f / R.l);
         }
         __syncthreads();
-        const float *x = P.scores + ((long long)g * M + r0) * P.own.cap + t0 + threadIdx.x;
+        const float *x = P.scores + ((long long)g * M + r0) * P.own.cap + t0;
         for (int r = 0; r < min(M - r0, 64); ++r, x += P.own.cap) {
             const float2 st = s_row[r];
+            float w[C];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (t0 + j * kAtCombine + (int)threadIdx.x < keys) {
-                    const float w = x[j * kAtCombine];
-                    if (w != -INFINITY) sum[j] = fmaf(ex2(w - st.x), st.y, sum[j]);
-                }
+            for (int j = 0; j < C; ++j) w[j] = t0 + j * kAtCombine < keys ? x[j * kAtCombine] : -INFINITY;
+#pragma unroll
+            for (int j = 0; j < C; ++j)
+                if (w[j] != -INFINITY) sum[j] = fmaf(ex2(w[j] - st.x), st.y, sum[j]);
         }
     }
+    float *acc = P.own.acc + (long long)g * P.own.cap + t0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int t = t0 + j * kAtCombine + threadIdx.x;
-        if (t < keys) P.own.acc[(long long)g * P.own.cap + t] += sum[j];
-    }
+    for (int j = 0; j < C; ++j)
+        if (t0 + j * kAtCombine < keys) acc[j * kAtCombine] += sum[j];
 }
 
 }  // namespace pgb
