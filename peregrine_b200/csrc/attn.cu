@@ -102,7 +102,7 @@ int attn_ctas(int D, int rt, int sms) {
 }
 
 // Shapes and the scratch's layout from the description of a call; bytes needed, or 0 for numbers past the kernels' range.
-size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, int rows, bool wide_weights, int sms, char *work) {
+size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, int rows, int sms, char *work) {
     const long long m_own = (long long)rows * (H / own.n_kv), m_pre = (long long)S * (H / own.n_kv);
     P->G = H / own.n_kv;
     const int rt = row_tile(rows, H, own.n_kv);
@@ -113,12 +113,11 @@ size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, i
     P->mt_own = (int)mt_own;
     P->mt_pre = (int)mt_pre;
     P->ctas = attn_ctas(own.D, rt, sms);
-    P->tc_keys = own.D == 256 || wide_weights ? 64 : 128;
     P->tc_rows = own.D == 256 ? 128 : 256;
     P->tc_ctas = sms;
-    P->tc_pre = m_pre > kTcRows && prefix_len >= P->tc_keys;
-    P->tc_own = m_own > kTcRows && own.cap >= P->tc_keys;
-    P->cut_pre = P->tc_pre ? prefix_len / P->tc_keys * P->tc_keys : 0;
+    P->tc_pre = m_pre > kTcRows && prefix_len >= kTcKeys;
+    P->tc_own = m_own > kTcRows && own.cap >= kTcKeys;
+    P->cut_pre = P->tc_pre ? prefix_len / kTcKeys * kTcKeys : 0;
     P->tc2_pre = own.D < 256 && m_pre <= 128;
     P->tc2_own = own.D < 256 && m_own <= 128;
     P->tcm_pre = P->tc_pre ? (int)((m_pre + P->tc_rows - 1) / P->tc_rows) : 0;
@@ -200,7 +199,7 @@ struct AttnLaunch {
         if (!opt_in(split, kSmem)) return 0;
         if (P.tc_pre || P.tc_own) {
             using T = TcShape<D, BF16, F32>;
-            static_assert(T::ROWS == (D == 256 ? 128 : 256) && T::N == (D == 256 || (BF16 && F32) ? 64 : 128), "as planned");
+            static_assert(T::ROWS == (D == 256 ? 128 : 256), "as planned");
             auto tc = attn_tc_kernel<D, BF16, F32>;
             if (!opt_in(tc, T::SMEM)) return 0;
             tc<<<dim3(P.tc_ctas), T::THREADS, T::SMEM, stream>>>(P, maps[0], maps[1], maps[2], maps[3]);
@@ -272,8 +271,7 @@ PGB_EXPORT size_t coli_cuda_pipe_attention_workspace(int device, int S, int H, c
     if (prefix_len < 0 || H % kv.n_kv || rows_per_seq > 64) return (size_t)refuse("%s: shape", what);
     if (!ctx_of(device, &c)) return (size_t)refuse("%s: device %d is not initialised", what, device);
     AttnArgs P{};
-    const size_t n0 = attn_plan(&P, kv, S, H, prefix_len, rows_per_seq, false, c.sms, nullptr);
-    const size_t n1 = attn_plan(&P, kv, S, H, prefix_len, rows_per_seq, true, c.sms, nullptr), need = n0 > n1 ? n0 : n1;
+    const size_t need = attn_plan(&P, kv, S, H, prefix_len, rows_per_seq, c.sms, nullptr);
     return need ? need : (size_t)refuse("%s: too many rows and heads", what);
 }
 
@@ -312,7 +310,7 @@ PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, 
     P.mask = reinterpret_cast<const unsigned long long *>(mask_dev);
     P.scale2 = scale * 1.4426950408889634f;
     if (!ctx_of(device, &c)) return refuse("%s: device %d is not initialised", what, device);
-    const size_t need = attn_plan(&P, P.own, S, H, prefix_len, rows_per_seq, out_f32 && own->dtype == 1, c.sms, static_cast<char *>(work_dev));
+    const size_t need = attn_plan(&P, P.own, S, H, prefix_len, rows_per_seq, c.sms, static_cast<char *>(work_dev));
     if (!need) return refuse("%s: too many rows and heads", what);
     if (work_bytes < need) return refuse("%s: %zu bytes of workspace, %zu are needed", what, work_bytes, need);
     P.err = c.err;

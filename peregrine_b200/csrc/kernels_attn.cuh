@@ -22,6 +22,7 @@ namespace pgb {
 constexpr int kAtKeys = 64;      // keys of a tile
 constexpr int kAtThreads = 160;  // 4 warps with 16 keys of a tile each, one that issues the copies
 constexpr int kAtCombine = 128;
+constexpr int kTcKeys = 64;  // keys of a tile of the tensor-memory kernel
 constexpr int kAtChunk = 1024;  // slots whose weights one CTA adds up
 
 struct AttnArgs {
@@ -37,8 +38,7 @@ struct AttnArgs {
     float scale2;                // scale * log2(e)
     int ctas;                    // CTAs that share the line of tiles
     int mt_pre, mt_own;          // row tiles of a problem (mt_pre 0: no prefix)
-    // the tensor-memory kernel: tiles of tc_keys keys that every row of a problem sees
-    int tc_keys;           // 64 or 128
+    // the tensor-memory kernel: tiles of 64 keys that every row of a problem sees
     int tc_pre, tc_own;    // whether it takes such tiles of the prefix, of the own slots
     int cut_pre;           // keys of the prefix that it takes
     int tc_ctas, tc_rows;  // its CTAs, rows of one of its partials
@@ -73,7 +73,7 @@ __device__ __forceinline__ int own_keys(const AttnArgs &P, int b) {
 __device__ __forceinline__ int own_cut(const AttnArgs &P, int b) {
     if (!P.tc_own) return 0;
     const int base = P.base[b];
-    return base < 0 ? 0 : min(base, P.own.cap) / P.tc_keys * P.tc_keys;
+    return base < 0 ? 0 : min(base, P.own.cap) / kTcKeys * kTcKeys;
 }
 // New slots that row i of a sequence sees, a bit each.
 __device__ __forceinline__ unsigned long long row_mask(const AttnArgs &P, int row, int i) {
@@ -108,10 +108,11 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
 }
 
 // Weights enter the second product in 16-bit terms.  A 16-bit output needs one (its own rounding is as large).  An fp32
-// output takes as many as give it 22 bits: two of f16, three of bf16.  f16 weights are scaled by 2^10 so that their lower term
-// stays a normal number down to weights of 2^-13 of the row's largest; l carries the same factor, so it cancels.
+// output takes as many as give it 22 bits: two of f16, three of bf16.  f16 weights are scaled by 2^6 against underflow of
+// their lower term (below 2^-24): with the 2^8 that the maximum may lag behind they stay below 2^15; l carries the same factor, so it cancels.
 template <bool BF16>
-constexpr float kAtLift = BF16 ? 0.0f : 10.0f;
+constexpr float kAtLift = BF16 ? 0.0f : 6.0f;
+constexpr float kAtLag = 8.0f;  // log2 by which a row's maximum may grow before o, l and m are rescaled
 template <bool BF16, bool F32>
 constexpr int kAtTerms = F32 ? (BF16 ? 3 : 2) : 1;
 
@@ -299,7 +300,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &P, const AttnAt &a, At
             }
         }
     }
-    // The maximum is only moved when it has grown by 2^4: it has to keep the weights in range, and cancels in o / l.
+    // The maximum only has to keep the weights in range, and cancels in o / l.
     float f[J];
     bool moved = false;
 #pragma unroll
@@ -308,7 +309,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &P, const AttnAt &a, At
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         f[j] = 1.0f;
-        if (top > A.m[j] + 4.0f) {
+        if (top > A.m[j] + kAtLag) {
             f[j] = ex2(A.m[j] - top);
             A.m[j] = top;
             A.l[j] *= f[j];

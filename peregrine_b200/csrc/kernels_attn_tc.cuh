@@ -2,10 +2,12 @@
 //
 // A CTA holds two tiles of 128 query vectors in shared memory and streams tiles of keys and values past them:
 //     S = Q K^T (tensor memory) -> weights 2^(x - m), written over S as the A operand -> O += P V (tensor memory)
-// One thread of a softmax warp owns one row (its TMEM lane), so a row's maximum and sum need no exchange.  The two tiles
+// Two threads own a row (its TMEM lane), 32 columns of a tile each: with one, the warps that form weights are too few to hide
+// their own latencies (measured: 1800 cycles a tile of 64 keys, 1050 with two).  The two row tiles
 // alternate: while one's weights are formed the tensor unit works for the other.  A 128 x 128 tile takes the tensor unit
-// 2 x 512 cycles (D = 128) and the exponential unit (16 a cycle) 1024, so neither can wait for the other.  O is rescaled
-// only when a row's maximum has grown by 2^4 since it was last set: m only has to keep weights in range, and cancels in
+// 2 x 512 cycles (D = 128) and the exponential unit (16 a cycle) 1024, so neither can wait for the other; S has two buffers
+// where they fit, so that the next scores are there when a tile's weights are done.  O is rescaled
+// only when a row's maximum has grown by 2^8 since it was last set: m only has to keep weights in range, and cancels in
 // O / l.  With at most 128 row vectors both tiles hold the same ones and the key tiles go to them in turn.  D = 256 has
 // no room for a second O: there one tile alternates between two S.
 //
@@ -16,28 +18,45 @@
 
 namespace pgb {
 
+// Tiles that a change of the problem costs a CTA (query vectors, first and last tile, its partial result): on the line every
+// (problem, row tile) begins with so many empty ones.
+constexpr int kTcEmpty = 8;
+
 template <int D, bool BF16, bool F32>
 struct TcShape {
-    static constexpr int TILES = D == 256 ? 1 : 2;    // row tiles of a CTA, a softmax warpgroup each
-    static constexpr int BUFS = D == 256 ? 2 : 1;     // S buffers of a row tile
+    static constexpr int TILES = D == 256 ? 1 : 2;  // row tiles of a CTA, 8 softmax warps each
     static constexpr int TERMS = kAtTerms<BF16, F32>;
-    static constexpr int N = D == 256 || TERMS == 3 ? 64 : 128;  // keys of a tile
-    // A buffer has 128 columns.  32 keys of weights take 16 columns a term; three terms outgrow the S they replace,
-    // which then sits in the upper half.
+    // S buffers of a row tile, and their columns.  32 keys of weights take 16 columns a term; three terms outgrow the S that
+    // they replace, which then sits in the upper half of a larger buffer.
+    static constexpr int BUFS = D == 256 || TERMS < 3 ? 2 : 1;
+    static constexpr int BUF_COLS = D < 256 && TERMS < 3 ? 64 : 128;
     static constexpr int S_COL = TERMS == 3 ? 64 : 0;
-    static constexpr int O_COL = TILES * BUFS * 128;
+    static constexpr int O_COL = 256;
+    static_assert(TILES * BUFS * BUF_COLS == 256 && O_COL + TILES * D <= 512, "columns");
+    static constexpr int N = kTcKeys;
     static constexpr int Q_BYTES = 128 * D * 2, TILE_BYTES = N * D * 2;
-    static constexpr int FIT = (232448 - 3072 - TILES * Q_BYTES) / TILE_BYTES;
+    static constexpr int FIT = (232448 - 5120 - TILES * Q_BYTES) / TILE_BYTES;
     static constexpr int SLOTS = FIT > 12 ? 12 : FIT;
     static constexpr int SMEM = 1024 + TILES * Q_BYTES + SLOTS * TILE_BYTES;
-    static constexpr int THREADS = TILES * 128 + 64;
+    static constexpr int THREADS = TILES * 256 + 64;  // softmax, copies, matrix instructions
     static constexpr int ROWS = TILES * 128;
 };
 
+// A place on the line; tiles and tile count the empty ones.
 struct TcAt {
     int seq, kvh, mt, tile, tiles;
 };
-__device__ __forceinline__ int tc_tiles(const AttnArgs &P, int b) { return own_cut(P, b) / P.tc_keys; }
+__device__ __forceinline__ int tc_tiles(const AttnArgs &P, int b) {
+    const int n = own_cut(P, b) / kTcKeys;
+    return n ? n + kTcEmpty : 0;
+}
+// The key tiles [t0, t0 + n) of the place's (problem, row tile) that lie in the next `left` tiles of the line; takes them off.
+__device__ __forceinline__ int tc_segment(const TcAt &a, int &left, int &t0) {
+    const int v = min(left, a.tiles - a.tile), t1 = a.tile + v - kTcEmpty;
+    left -= v;
+    t0 = max(a.tile - kTcEmpty, 0);
+    return max(t1 - t0, 0);
+}
 // Moves to the next (problem, row tile) with tiles.
 __device__ __forceinline__ void tc_next(const AttnArgs &P, TcAt &a) {
     a.tile = 0;
@@ -56,6 +75,52 @@ __device__ __forceinline__ void tc_next(const AttnArgs &P, TcAt &a) {
 
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {  // 128-byte swizzle, 8-row groups 1024 bytes apart
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void tile_sync(int w) { asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory"); }  // the warps of a row tile
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// Pairs of fp32 values, an operation on both at once.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^y of both halves for finite y: 2^n 2^f with n the nearest whole number, found by adding 1.5 x 2^23, and the Taylor sum of
+// e^(f ln 2), |f| <= 1/2, to the power DEG: off by (ln 2 / 2)^(DEG + 1) / (DEG + 1)!, 4.2e-5, 2.4e-6 or 1.2e-7 for 4, 5, 6.
+// Below 2^-126 the result stays there.
+template <int DEG>
+__device__ __forceinline__ void exp2_poly(uint64_t y, float &lo, float &hi) {
+    constexpr float kC[7] = {1.0f,           0.69314718056f,  0.24022650696f, 0.05550410866f,
+                             0.00961812911f, 0.00133335581f, 0.000154035304f};  // ln(2)^k / k!
+    float a, b;
+    unpack2(y, a, b);
+    a = fmaxf(a, -126.0f);
+    b = fmaxf(b, -126.0f);
+    y = pack2(a, b);
+    const uint64_t t = add2(y, pack2(12582912.0f, 12582912.0f));
+    const uint64_t f = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), y);
+    uint64_t p = pack2(kC[DEG], kC[DEG]);
+#pragma unroll
+    for (int k = DEG - 1; k >= 0; --k) p = fma2(p, f, pack2(kC[k], kC[k]));
+    float ta, tb;
+    unpack2(t, ta, tb);
+    unpack2(p, a, b);
+    lo = __uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23));
+    hi = __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23));
 }
 // `i`-th user of a ring of n: its place and the parity of its turn.
 template <int n>
@@ -80,37 +145,31 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     extern __shared__ __align__(128) uint8_t tc_smem_raw[];
     __shared__ __align__(8) unsigned long long s_bar[2 * T::SLOTS + 3 * T::TILES + 2 * T::TILES * T::BUFS];
     __shared__ uint32_t s_tmem;
+    __shared__ float s_top[2][T::TILES][2][128];  // a row's two maxima, by turns
     __shared__ int s_fail;
     const int tid = threadIdx.x, warp = tid >> 5, c = blockIdx.x;
     griddep_launch_dependents();
-    if (tid == 0) s_fail = 0;
-    const int nkv = P.own.n_kv, per_seq = nkv * P.tcm_own, tp = P.tc_pre ? P.cut_pre / N : 0;
-    const long long line_pre = (long long)nkv * P.tcm_pre * tp;
-    long long first, end;
-    int seq = 0, off = 0;
-    if (!line_share<T::THREADS / 32>(P.own.n_seq, [&](int b) { return tc_tiles(P, b); }, per_seq, line_pre, P.tc_ctas, first, end, seq,
-                                     off))
-        return;
     uint8_t *base = tc_smem_raw + ((1024 - (smem_u32(tc_smem_raw) & 1023)) & 1023);
     const uint32_t q_s = smem_u32(base), ring_s = q_s + T::TILES * T::Q_BYTES;
     const uint32_t full = smem_u32(s_bar), empty = full + 8 * T::SLOTS, qfull = empty + 8 * T::SLOTS, odone = qfull + 8 * T::TILES,
                    sfull = odone + 8 * T::TILES, pfull = sfull + 8 * T::TILES * T::BUFS,
                    pvdone = pfull + 8 * T::TILES * T::BUFS;
     volatile int *fail = &s_fail;
+    constexpr int kProducer = T::TILES * 8, kIssuer = kProducer + 1;
     if (tid == 0) {
+        s_fail = 0;
         for (int i = 0; i < 2 * T::SLOTS; ++i) mbar_init(full + 8 * i, 1);
         for (int i = 0; i < T::TILES; ++i) {
-            mbar_init(qfull + 8 * i, 4);
+            mbar_init(qfull + 8 * i, 8);
             mbar_init(odone + 8 * i, 1);
             mbar_init(pvdone + 8 * i, 1);
         }
         for (int i = 0; i < T::TILES * T::BUFS; ++i) {
             mbar_init(sfull + 8 * i, 1);
-            mbar_init(pfull + 8 * i, 4);
+            mbar_init(pfull + 8 * i, 8);
         }
         fence_mbar_init();
     }
-    constexpr int kProducer = T::TILES * 4, kIssuer = kProducer + 1;
     if (warp == kIssuer) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -119,8 +178,17 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = s_tmem;
+    const int nkv = P.own.n_kv, per_seq = nkv * P.tcm_own, tp = P.tc_pre ? P.cut_pre / N + kTcEmpty : 0;
+    const long long line_pre = (long long)nkv * P.tcm_pre * tp;
+    long long first = 0, end = 0;
+    int seq = 0, off = 0;
+    if (!line_share<T::THREADS / 32>(P.own.n_seq, [&](int b) { return tc_tiles(P, b); }, per_seq, line_pre, P.tc_ctas, first, end, seq,
+                                     off))
+        first = end = 0;
     TcAt at;
-    if (first < line_pre) {
+    if (first == end) {
+        at = TcAt{0, 0, 0, 0, 0};
+    } else if (first < line_pre) {
         const int u = (int)(first / tp);
         at = TcAt{-1, u / P.tcm_pre, u % P.tcm_pre, (int)(first % tp), tp};
     } else {
@@ -130,13 +198,14 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
         at = TcAt{seq, u / P.tcm_own, u % P.tcm_own, (int)(in % tiles), tiles};
     }
     int left = (int)(end - first);
-
     if (warp == kProducer) {
         // ================================================================ copies: K and V of a tile in boxes of 64 keys x 64 dims
         if (elect_one()) {
             RingAt<T::SLOTS> r;
-            for (; left > 0 && !*fail; tc_next(P, at)) {
-                const int n = min(left, at.tiles - at.tile), s = at.seq < 0 ? 0 : at.seq;
+            bool begun = false;
+            while (left > 0 && !*fail) {
+                int t0;
+                const int n = tc_segment(at, left, t0), s = at.seq < 0 ? 0 : at.seq;
                 const CUtensorMap *mk = at.seq < 0 ? &pre_k : &own_k, *mv = at.seq < 0 ? &pre_v : &own_v;
                 for (int j = 0; j < n && !*fail; ++j)
 #pragma unroll
@@ -146,13 +215,16 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                         mbar_expect_tx(full + 8 * r.i, T::TILE_BYTES);
 #pragma unroll
                         for (int b = 0; b < DB; ++b)
-#pragma unroll
-                            for (int h = 0; h < N / 64; ++h)
-                                tma_load_4d(ring_s + r.i * T::TILE_BYTES + b * (N * 128) + h * 8192, v ? mv : mk, b * 64,
-                                            (at.tile + j) * N + h * 64, at.kvh, s, full + 8 * r.i);
+                            tma_load_4d(ring_s + r.i * T::TILE_BYTES + b * (N * 128), v ? mv : mk, b * 64, (t0 + j) * N, at.kvh, s, full + 8 * r.i);
                         r.skip(1);
+                        if (!begun && v) {
+                            // The query vectors' loads must not queue behind a ring full of tiles.  (With three tiles to come
+                            // the barrier stays in this phase until they do.)
+                            begun = true;
+                            if (n > 2) um_spin(qfull, 0u, fail);
+                        }
                     }
-                left -= n;
+                tc_next(P, at);
             }
         }
     } else if (warp == kIssuer) {
@@ -164,7 +236,8 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             RingAt<T::SLOTS> seg;  // the ring place of the segment's first K
             uint32_t qph = 0, pph[T::TILES][T::BUFS] = {};
             for (; left > 0 && !*fail; tc_next(P, at)) {
-                const int n = min(left, at.tiles - at.tile);
+                int t0;
+                const int n = tc_segment(at, left, t0);
                 const int two = T::TILES == 2 && (at.seq < 0 ? P.tc2_pre : P.tc2_own);
                 // tile i of row tile w is key tile `i` of the segment, or 2 i + w when they take turns
                 auto count = [&](int w) { return two ? (n + 1 - w) >> 1 : n; };
@@ -178,7 +251,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                     if (i == 0) um_spin(qfull + 8 * w, (qph >> w) & 1u, fail);
                     if (w == 0 || two) um_spin(full + 8 * r.i, r.ph, fail);
                     tmem_fence_after();
-                    const uint32_t d = tmem + (w * T::BUFS + i % T::BUFS) * 128 + T::S_COL;
+                    const uint32_t d = tmem + (w * T::BUFS + i % T::BUFS) * T::BUF_COLS + T::S_COL;
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
                         umma_f16_ss(d, desc_sw128(q_s + w * T::Q_BYTES + (k >> 2) * (128 * 128), 16) + (k & 3) * 2,
@@ -208,7 +281,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                         for (int k = 0; k < N / 16; ++k)
 #pragma unroll
                             for (int t = 0; t < T::TERMS; ++t)
-                                umma_f16_ts(tmem + T::O_COL + w * D, tmem + buf * 128 + (k >> 1) * (16 * T::TERMS) + t * 16 + (k & 1) * 8,
+                                umma_f16_ts(tmem + T::O_COL + w * D, tmem + buf * T::BUF_COLS + (k >> 1) * (16 * T::TERMS) + t * 16 + (k & 1) * 8,
                                             desc_sw128(ring_s + r.i * T::TILE_BYTES + k * 2048, N * 128), kIdescO, i > 0 || k > 0 || t > 0);
                         if (w == T::TILES - 1 || two) umma_commit(empty + 8 * r.i);
                         if (T::BUFS > 1) umma_commit(pvdone + 8 * w);
@@ -219,38 +292,47 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                     }
                 seg.skip(2 * n % T::SLOTS);
                 if ((2 * n / T::SLOTS) & 1) seg.ph ^= 1u;
-                left -= n;
             }
         }
     } else {
-        // ================================================================ softmax: one row of row tile w per thread
-        const int w = warp >> 2, lane = tid & 31, row = tid & 127;
+        // ================================================================ softmax: half a row of row tile w per thread
+        const int w = warp >> 3, hf = (warp >> 2) & 1, lane = tid & 31, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 TMEM lanes
         const uint32_t flip = P.scale2 < 0.0f ? 0x80008000u : 0u;  // the sign of the scale goes into Q: scores only need a positive one
         const float scale = fabsf(P.scale2);
+        int turn = 0;
         uint32_t sph[T::BUFS] = {}, oph = 0, pvph = 1;  // pvph: parity of the product before this tile's
         for (; left > 0; tc_next(P, at)) {
-            const int n = min(left, at.tiles - at.tile);
+            int t0;
+            const int n = tc_segment(at, left, t0);
+            if (n == 0) continue;  // empty tiles alone
             const int two = T::TILES == 2 && (at.seq < 0 ? P.tc2_pre : P.tc2_own);
             const int mine = two ? (n + 1 - w) >> 1 : n;
             const int M = (at.seq < 0 ? P.S : P.rows) * P.G, row0 = at.seq < 0 ? 0 : at.seq * P.rows;
             const int r = two ? at.mt * 128 + row : at.mt * T::ROWS + w * 128 + row;
             float m = -INFINITY, l = 0.0f;
             if (mine) {
-                const uint16_t *src = P.q + ((long long)(row0 + r / P.G) * P.H + at.kvh * P.G + r % P.G) * D;
-                uint8_t *to = base + w * T::Q_BYTES + row * 128;
+                // D / 8 lanes read a row together; a warp brings 16 of its 32 rows
+                constexpr int LPR = D / 8, RPI = 32 / LPR, B = 16 / RPI < 8 ? 16 / RPI : 8;
+                const int ch = lane % LPR, rl = (row & ~31) + hf * 16 + lane / LPR;
+                uint8_t *to = base + w * T::Q_BYTES + (ch >> 3) * (128 * 128);
+                int q = r - row + rl, div = q / P.G, rem = q - div * P.G;  // row vector, its row and head
+                const uint16_t *src = P.q + ((long long)row0 * P.H + at.kvh * P.G) * D + ch * 8;
 #pragma unroll
-                for (int c0 = 0; c0 < D / 8; c0 += 16) {
-                    constexpr int B = D / 8 < 16 ? D / 8 : 16;  // loads under way together
+                for (int i0 = 0; i0 < 16 / RPI; i0 += B) {
                     uint4 v[B];
 #pragma unroll
-                    for (int e = 0; e < B; ++e)
-                        v[e] = r < M ? *reinterpret_cast<const uint4 *>(src + (c0 + e) * 8) : make_uint4(0, 0, 0, 0);
+                    for (int e = 0; e < B; ++e) {
+                        v[e] = make_uint4(0, 0, 0, 0);
+                        if (q < M) v[e] = *reinterpret_cast<const uint4 *>(src + ((long long)div * P.H + rem) * D);
+                        q += RPI;
+                        for (rem += RPI; rem >= P.G; ++div) rem -= P.G;
+                    }
 #pragma unroll
                     for (int e = 0; e < B; ++e) {
-                        const int ch = c0 + e;
+                        const int k = rl + (i0 + e) * RPI;
                         v[e].x ^= flip, v[e].y ^= flip, v[e].z ^= flip, v[e].w ^= flip;
-                        *reinterpret_cast<uint4 *>(to + (ch >> 3) * (128 * 128) + (((ch & 7) ^ (row & 7)) << 4)) = v[e];
+                        *reinterpret_cast<uint4 *>(to + k * 128 + (((ch & 7) ^ (k & 7)) << 4)) = v[e];
                     }
                 }
                 fence_proxy_async();
@@ -259,33 +341,37 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             }
             for (int i = 0; i < mine; ++i) {
                 const int bi = i % T::BUFS, buf = w * T::BUFS + bi;
-                const uint32_t region = tmem + lanes + buf * 128;
+                const uint32_t region = tmem + lanes + buf * T::BUF_COLS;
                 um_spin(sfull + 8 * buf, sph[bi], fail);
                 sph[bi] ^= 1u;
                 tmem_fence_after();
-                float s[N];
-#pragma unroll
-                for (int q = 0; q < N / 32; ++q) tmem_ld32(region + T::S_COL + q * 32, s + q * 32);
-#pragma unroll
-                for (int q = 0; q < N / 32; ++q) tmem_wait_ld32(s + q * 32);
+                float s[32];
+                tmem_ld32(region + T::S_COL + hf * 32, s);
+                tmem_wait_ld32(s);
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int e = 4; e < N; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                for (int e = 4; e < 32; ++e) mx[e & 3] = max_nan(mx[e & 3], s[e]);
+                float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
+                // both halves of S have been read when both maxima are there: the weights may replace any of it
+                s_top[turn][w][hf][row] = top;
+                tile_sync(w);
+                top = max_nan(top, s_top[turn][w][hf ^ 1][row]);
+                turn ^= 1;
+                const bool plain = __all_sync(0xffffffffu, top < INFINITY);  // no NaN, no infinity
                 if (i == 0) {
                     m = top;
-                } else if (__any_sync(0xffffffffu, top > m + 4.0f)) {
+                } else if (__any_sync(0xffffffffu, top > m + kAtLag)) {
                     // O of this row tile is at rest: the product before was committed with these scores, or is waited for
                     if (T::BUFS > 1) {
                         um_spin(pvdone + 8 * w, pvph, fail);
                         tmem_fence_after();
                     }
-                    const float to = top > m + 4.0f ? top : m;
+                    const float to = top > m + kAtLag ? top : m;
                     const float f = to == m ? 1.0f : ex2(m - to);
                     m = to;
                     l *= f;
 #pragma unroll 1
-                    for (int d = 0; d < D; d += 32) {
+                    for (int d = hf * (D / 2); d < (hf + 1) * (D / 2); d += 32) {
                         float o[32];
                         tmem_ld32(tmem + lanes + T::O_COL + w * D + d, o);
                         tmem_wait_ld32(o);
@@ -301,19 +387,35 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                 pvph ^= 1u;
                 if (P.scores && at.seq >= 0 && r < M) {
                     float *x = P.scores + (((long long)at.seq * nkv + at.kvh) * M + r) * P.own.cap +
-                               (long long)(at.tile + (two ? 2 * i + w : i)) * N;
+                               (long long)(t0 + (two ? 2 * i + w : i)) * N + hf * 32;
 #pragma unroll
-                    for (int e = 0; e < N; ++e) x[e] = s[e] * scale;
+                    for (int e = 0; e < 32; ++e) x[e] = s[e] * scale;
                 }
                 const float ms = (m == -INFINITY ? 0.0f : m) - kAtLift<BF16>;
-                float sum[4] = {};
+                const uint64_t scales = pack2(scale, scale), shift = pack2(-ms, -ms);
+                uint64_t sums[2] = {0, 0};
+                {
+                    float *x = s;
+                    // Three pairs of eight go to a polynomial: the exponential unit alone would take 1024 cycles for a
+                    // 128 x 128 tile, as long as both products, and it serves both row tiles.
+                    if (plain) {
 #pragma unroll
-                for (int q = 0; q < N / 32; ++q) {
-                    float *x = s + q * 32;
+                        for (int e = 0; e < 16; ++e) {
+                            const uint64_t y = fma2(pack2(x[2 * e], x[2 * e + 1]), scales, shift);
+                            if ((e & 7) < 3) {
+                                exp2_poly<T::TERMS == 1 ? (BF16 ? 4 : 5) : 6>(y, x[2 * e], x[2 * e + 1]);
+                            } else {
+                                unpack2(y, x[2 * e], x[2 * e + 1]);
+                                x[2 * e] = ex2(x[2 * e]);
+                                x[2 * e + 1] = ex2(x[2 * e + 1]);
+                            }
+                            sums[e & 1] = add2(sums[e & 1], pack2(x[2 * e], x[2 * e + 1]));
+                        }
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        x[e] = ex2(fmaf(x[e], scale, -ms));
-                        sum[e & 3] += x[e];
+                        for (int e = 0; e < 32; ++e) x[e] = ex2(fmaf(x[e], scale, -ms));
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) sums[e & 1] = add2(sums[e & 1], pack2(x[2 * e], x[2 * e + 1]));
                     }
 #pragma unroll
                     for (int t = 0; t < T::TERMS; ++t) {
@@ -326,10 +428,14 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                                 x[2 * e + 1] -= high16<BF16>(u[e]);
                             }
                         }
-                        tmem_st16(region + q * (16 * T::TERMS) + t * 16, u);
+                        tmem_st16(region + hf * (16 * T::TERMS) + t * 16, u);
                     }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                {
+                    float a, b;
+                    unpack2(add2(sums[0], sums[1]), a, b);
+                    l += a + b;
+                }
                 tmem_wait_st();
                 tmem_fence_before();
                 __syncwarp();
@@ -338,32 +444,46 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             // the segment's partial result
             const int unit = at.seq < 0 ? at.kvh * P.tcm_pre + at.mt
                                         : nkv * P.tcm_pre + (at.seq * nkv + at.kvh) * P.tcm_own + at.mt;
-            const long long to = P.tc_row0 + ((long long)unit + c) * T::ROWS + w * 128 + row;
-            if (tid == 0 && at.tile == 0) P.tc_cta_of[unit].x = c;
-            if (tid == 0 && at.tile + n == at.tiles) P.tc_cta_of[unit].y = c;
+            const long long to = P.tc_row0 + ((long long)unit + c) * T::ROWS + w * 128;
+            if (tid == 0 && t0 == 0) P.tc_cta_of[unit].x = c;
+            if (tid == 0 && t0 + n + kTcEmpty == at.tiles) P.tc_cta_of[unit].y = c;
             if (mine) {
                 um_spin(odone + 8 * w, oph, fail);
                 oph ^= 1u;
                 tmem_fence_after();
             }
-            if (r < M) P.ml[to] = make_float2(m, l);
-#pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-                float o[32];
+            // the halves' sums meet (the maxima are the same); nobody reads the other turn's any more
+            s_top[turn][w][hf][row] = l;
+            tile_sync(w);
+            if (hf == 0 && r < M) P.ml[to + row] = make_float2(m, l + s_top[turn][w][1][row]);
+            turn ^= 1;
+            // A thread has a row's dims, a store wants a row's dims in neighbouring lanes: 32 rows x 16 dims at a time turn in
+            // the shared memory of this row tile's query vectors, whose products are done.
+            uint8_t *swap = base + w * T::Q_BYTES + (warp & 7) * 2048;
+#pragma unroll 2
+            for (int d = hf * (D / 2); d < (hf + 1) * (D / 2); d += 16) {
+                float o[16];
                 if (mine) {
-                    tmem_ld32(tmem + lanes + T::O_COL + w * D + d, o);
-                    tmem_wait_ld32(o);
+                    tmem_ld16(tmem + lanes + T::O_COL + w * D + d, o);
+                    tmem_wait_ld16(o);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                    for (int e = 0; e < 16; ++e) o[e] = 0.0f;
                 }
-                if (r < M)
+                __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4 *>(P.part + to * D + d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                for (int e = 0; e < 4; ++e)
+                    *reinterpret_cast<float4 *>(swap + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int rr = e * 8 + (lane >> 2), ch = lane & 3;
+                    const float4 v = *reinterpret_cast<const float4 *>(swap + rr * 64 + ((ch ^ ((rr >> 1) & 3)) << 4));
+                    if (r - lane + rr < M) *reinterpret_cast<float4 *>(P.part + (to + (row & ~31) + rr) * D + d + ch * 4) = v;
+                }
             }
+            tile_sync(w);  // before new query vectors replace what another warp still turns
             tmem_fence_before();
-            left -= n;
         }
     }
     __syncwarp();
