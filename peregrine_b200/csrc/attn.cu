@@ -76,15 +76,27 @@ int by_type(int D, int dtype, F &&f) {  // f.template operator()<D, BF16>()
 }
 
 struct NormRopeLaunch {
-    const NormRopeArgs &P;
+    NormRopeArgs &P;
     int S, sms;
     cudaStream_t stream;
     template <int D, bool BF16>
     int operator()() const {
-        // a CTA takes all heads of a row once the rows alone fill the device a few times over
-        const int per_cta = kNrWarps * (256 / D), groups = (P.H + 2 * P.kv.n_kv + per_cta - 1) / per_cta;
-        const int split = S >= 8 * sms ? 1 : groups;
-        norm_rope_kernel<D, BF16><<<dim3(S, split < 65535 ? split : 65535), kNrWarps * 32, 0, stream>>>(P);
+        // Items of `per` steps of a row are dealt to the warps in rounds; the row's angles cost an item about two steps.
+        const int warps = 2 * kNrWarps * sms, steps = ((P.H + 2 * P.kv.n_kv) * D + 255) / 256;
+        long long best = -1;
+        for (int per = 1; per <= steps; ++per) {
+            const long long items = (long long)S * ((steps + per - 1) / per), cost = (items + warps - 1) / warps * (per + 2);
+            if (best < 0 || cost < best) {
+                best = cost;
+                P.per = per;
+            }
+        }
+        P.rows = S;
+        P.steps = steps;
+        P.parts = (steps + P.per - 1) / P.per;
+        if ((long long)S * P.parts > 0x7fffffffll) return refuse("pipe_qk_norm_rope: too many rows and heads");
+        const long long need = ((long long)S * P.parts + kNrWarps - 1) / kNrWarps;
+        norm_rope_kernel<D, BF16><<<dim3((unsigned)(need < 2 * sms ? need : 2 * sms)), kNrWarps * 32, 0, stream>>>(P);
         return launched("qk_norm_rope launch");
     }
 };
@@ -357,17 +369,30 @@ PGB_EXPORT int coli_cuda_pipe_kv_evict(int device, const ColiCudaKv *dst, const 
     if (!ctx_of(device, &c)) return refuse("%s: device %d is not initialised", what, device);
     DeviceGuard g(c.device);
     if (!g.ok()) return refuse("%s: device %d cannot be selected", what, device);
-    evict_select_kernel<<<dim3((unsigned)groups), kEvThreads, 0, c.stream>>>(P);
-    if (!launched("kv_evict select launch")) return 0;
-    const int per_cta = 256 / (src->D / 8);
+    if (src->cap > kEvCluster * kEvPartMost) {
+        evict_select_kernel<<<dim3((unsigned)groups), kEvThreads, 0, c.stream>>>(P);
+        if (!launched("kv_evict select launch")) return 0;
+    } else {
+        const int parts = src->cap <= kEvAlone ? 1 : kEvCluster, most = (((src->cap + parts - 1) / parts) + 7) & ~7, smem = most * 6;
+        auto kernel = parts == 1 ? evict_select_cluster_kernel<1> : evict_select_cluster_kernel<kEvCluster>;
+        if (!opt_in(kernel, smem)) return 0;
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)parts;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3((unsigned)(groups * parts));
+        cfg.blockDim = dim3(kEvPartThreads);
+        cfg.dynamicSmemBytes = (size_t)smem;
+        cfg.stream = c.stream;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, kernel, (const EvictArgs)P, most);
+        if (!launched("kv_evict select launch")) return 0;
+    }
+    const int per_cta = 4 * 256 / (src->D / 8);
     const long long most = ((long long)keep + per_cta - 1) / per_cta, want = (16ll * c.sms + groups - 1) / groups;
     P.chunks = (int)(most < want ? most : want);
-    const dim3 grid((unsigned)(groups * P.chunks));
-    if (src->D == 64)
-        evict_move_kernel<64><<<grid, 256, 0, c.stream>>>(P);
-    else if (src->D == 128)
-        evict_move_kernel<128><<<grid, 256, 0, c.stream>>>(P);
-    else
-        evict_move_kernel<256><<<grid, 256, 0, c.stream>>>(P);
-    return launched("kv_evict move launch");
+    auto move = src->D == 64 ? evict_move_kernel<64> : src->D == 128 ? evict_move_kernel<128> : evict_move_kernel<256>;
+    return launch_early(move, (unsigned)(groups * P.chunks), 256, 0, c.stream, "kv_evict move launch", P);
 }

@@ -55,6 +55,7 @@ __device__ __forceinline__ int block_scan(int v, int *s_warp, int &total) {
     return before + x - v;
 }
 
+// One CTA for caches whose keys do not fit into a cluster's shared memory: every sweep forms them anew.
 __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArgs P) {
     __shared__ int s_warp[32], s_hist[256], s_digit, s_above, s_last;
     const int seq = blockIdx.x / P.src.n_kv;
@@ -148,30 +149,240 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
     }
 }
 
-// Moves the selected rows: 16 bytes a lane, D / 8 lanes for a row of k and as many for v.
+// The same on a cluster of C CTAs (kEvCluster, or 1 for short caches) per (sequence, kv head): every CTA keeps the keys of its
+// part of the slots in shared memory, histograms and counts are read across the cluster.  One CTA alone reads at about
+// 100 GB/s and sweeps 40000 slots six times in 108 us; eight take 8.
+constexpr int kEvCluster = 8, kEvPartThreads = 512, kEvPartMost = 32768;  // slots of a CTA at the most
+constexpr int kEvAlone = 4096;                                            // up to here one CTA is a cluster
+
+template <int C>
+__device__ __forceinline__ void cluster_sync() {
+    if (C == 1) {
+        __syncthreads();
+    } else {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+}
+template <int C>
+__device__ __forceinline__ int cluster_ld(const int *p, int rank) {  // *p of CTA `rank` of the cluster
+    if (C == 1) return *p;
+    uint32_t a, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return (int)v;
+}
+template <int C>
+__device__ __forceinline__ int cluster_ld16(const uint16_t *p, int rank) {
+    if (C == 1) return *p;
+    uint32_t a;
+    uint16_t v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+    return v;
+}
+
+template <int C>
+__global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(const EvictArgs P, int part_most) {
+    constexpr int W = kEvPartThreads / 32;
+    extern __shared__ __align__(16) uint32_t ev_key[];
+    uint16_t *surv = reinterpret_cast<uint16_t *>(ev_key + part_most);  // the part's kept slots behind `keep`, in order
+    __shared__ int s_hist[2][256], s_last, s_ties, s_far, s_holes, s_digit, s_above, s_warp[3][W];
+    const int rank = C == 1 ? 0 : blockIdx.x % C, g = blockIdx.x / C, seq = g / P.src.n_kv;
+    griddep_launch_dependents();
+    int len = P.len[seq];
+    if (len < 0) return;
+    len = min(len, P.src.cap);
+    const int count = min(len, P.keep), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int *index = P.index + (long long)g * P.keep;
+    for (int i = count + rank * kEvPartThreads + tid; i < P.keep; i += C * kEvPartThreads) index[i] = -1;
+    if (len <= P.keep) {
+        for (int i = rank * kEvPartThreads + tid; i < count; i += C * kEvPartThreads) index[i] = i;
+        return;
+    }
+    const int part = (len + C - 1) / C, lo = min(rank * part, len), n = min(part, len - lo);
+    const float *acc = P.src.acc + (long long)g * P.src.cap + lo;
+    const int *pos = P.src.pos + (long long)g * P.src.cap + lo;
+    if (tid == 0) s_last = INT_MIN, s_ties = s_far = s_holes = 0;
+    if (tid < 256) s_hist[0][tid] = s_hist[1][tid] = 0;
+    __syncthreads();
+    int last = INT_MIN;
+#pragma unroll 4
+    for (int i = tid; i < n; i += kEvPartThreads) last = max(last, pos[i]);
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0) atomicMax(&s_last, last);
+    cluster_sync<C>();
+#pragma unroll
+    for (int r = 0; r < C; ++r) last = max(r ? last : INT_MIN, cluster_ld<C>(&s_last, r));
+#pragma unroll 4
+    for (int i = tid; i < n; i += kEvPartThreads) ev_key[i] = evict_key(acc[i], pos[i], last, P.sinks, P.recent);
+    __syncthreads();
+    // radix select: `prefix` = the digits of the count-th largest key found so far, `want` = its rank among equals
+    uint32_t prefix = 0;
+    int want = count;
+#pragma unroll 1
+    for (int pass = 0; pass < 4; ++pass) {
+        const int shift = 24 - 8 * pass;
+        int *hist = s_hist[pass & 1];
+        for (int i0 = warp * 32; i0 < n; i0 += kEvPartThreads) {
+            const int i = i0 + lane;
+            const uint32_t key = i < n ? ev_key[i] : 0u;
+            const bool in = i < n && (pass == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
+            const int digit = in ? (int)((key >> shift) & 255) : -1;
+            const uint32_t same = __match_any_sync(0xffffffffu, digit);  // weights share their leading digits
+            if (in && (same & ((1u << lane) - 1)) == 0) atomicAdd(&hist[digit], __popc(same));
+        }
+        cluster_sync<C>();
+        int mine = 0;
+        if (tid < 256) {
+#pragma unroll
+            for (int r = 0; r < C; ++r) mine += cluster_ld<C>(&hist[255 - tid], r);
+            s_hist[(pass + 1) & 1][tid] = 0;  // read by all before the last barrier but one
+        }
+        int x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) s_warp[0][warp] = x;
+        __syncthreads();
+        int above = x - mine;  // keys of a larger digit
+        for (int w = 0; w < min(warp, 8); ++w) above += s_warp[0][w];
+        if (tid < 256 && above < want && above + mine >= want) {
+            s_digit = 255 - tid;
+            s_above = above;
+        }
+        __syncthreads();
+        prefix |= (uint32_t)s_digit << shift;
+        want -= s_above;
+    }
+    // Warps own runs of the part: `want` of the slots with this very key are kept, the lowest ones.
+    const int run = (n + W * 32 - 1) / (W * 32) * 32, a0 = min(warp * run, n), a1 = min(a0 + run, n);
+    int ties = 0;
+    for (int i = a0 + lane; i < a0 + run; i += 32) ties += i < a1 && ev_key[i] == prefix;
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    if (lane == 0) {
+        s_warp[0][warp] = ties;
+        atomicAdd(&s_ties, ties);
+    }
+    cluster_sync<C>();
+    int before = 0;
+    for (int r = 0; r < rank; ++r) before += cluster_ld<C>(&s_ties, r);
+    for (int w = 0; w < warp; ++w) before += s_warp[0][w];
+    const uint32_t below = (1u << lane) - 1;
+    int far = 0, holes = 0;
+    for (int i0 = a0, t = before; i0 < a1; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t key = i < a1 ? ev_key[i] : 0u;
+        const uint32_t tb = __ballot_sync(0xffffffffu, i < a1 && key == prefix);
+        const bool kept = i < a1 && (key > prefix || (key == prefix && t + __popc(tb & below) < want));
+        t += __popc(tb);
+        far += __popc(__ballot_sync(0xffffffffu, kept && lo + i >= P.keep));
+        holes += __popc(__ballot_sync(0xffffffffu, i < a1 && !kept && lo + i < P.keep));
+    }
+    if (lane == 0) {
+        s_warp[1][warp] = far;
+        s_warp[2][warp] = holes;
+        atomicAdd(&s_far, far);
+        atomicAdd(&s_holes, holes);
+    }
+    __syncthreads();
+    int f = 0, h = 0;
+    for (int w = 0; w < warp; ++w) {
+        f += s_warp[1][w];
+        h += s_warp[2][w];
+    }
+    for (int i0 = a0, t = before; i0 < a1; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t key = i < a1 ? ev_key[i] : 0u;
+        const uint32_t tb = __ballot_sync(0xffffffffu, i < a1 && key == prefix);
+        const bool kept = i < a1 && (key > prefix || (key == prefix && t + __popc(tb & below) < want));
+        t += __popc(tb);
+        const uint32_t fb = __ballot_sync(0xffffffffu, kept && lo + i >= P.keep);
+        if (kept && lo + i >= P.keep) surv[f + __popc(fb & below)] = (uint16_t)i;
+        f += __popc(fb);
+    }
+    cluster_sync<C>();
+    int fars[C];  // kept slots behind `keep` in the parts before the r-th
+    {
+        int sum = 0;
+#pragma unroll
+        for (int r = 0; r < C; ++r) {
+            fars[r] = sum;
+            sum += cluster_ld<C>(&s_far, r);
+            if (r < rank) h += cluster_ld<C>(&s_holes, r);
+        }
+    }
+    for (int i0 = a0, t = before; i0 < a1 && lo + i0 < P.keep; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t key = i < a1 ? ev_key[i] : 0u;
+        const uint32_t tb = __ballot_sync(0xffffffffu, i < a1 && key == prefix);
+        const bool kept = i < a1 && (key > prefix || (key == prefix && t + __popc(tb & below) < want));
+        t += __popc(tb);
+        const bool hole = i < a1 && !kept && lo + i < P.keep;
+        const uint32_t hb = __ballot_sync(0xffffffffu, hole);
+        if (hole) {
+            const int m = h + __popc(hb & below);
+            int r = 0, first = 0;
+#pragma unroll
+            for (int q = 1; q < C; ++q)
+                if (fars[q] <= m) r = q, first = fars[q];
+            index[lo + i] = r * part + cluster_ld16<C>(&surv[m - first], r);
+        } else if (kept && lo + i < P.keep) {
+            index[lo + i] = lo + i;
+        }
+        h += __popc(hb);
+    }
+    cluster_sync<C>();  // nobody leaves while its shared memory is read
+}
+
+// Moves the selected rows: 16 bytes a lane, D / 8 lanes for a row of k and of v, four rows under way at a time.
 template <int D>
 __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs P) {
-    constexpr int LPR = D / 8;
+    constexpr int LPR = D / 8, ROWS = 256 / LPR, U = 4;
     const int g = blockIdx.x / P.chunks, chunk = blockIdx.x % P.chunks, seq = g / P.src.n_kv, kvh = g % P.src.n_kv;
+    griddep_wait();
     const int len = P.len[seq];
     const int count = min(min(len, P.src.cap), P.keep);
     if (kvh == 0 && chunk == 0 && threadIdx.x == 0) P.new_len[seq] = min(len, P.keep);
     if (len < 0) return;
     const bool in_place = P.dst.k == P.src.k;
     const int sub = threadIdx.x / LPR, l = threadIdx.x % LPR;
-    const long long sb = (long long)seq * P.src.seq_stride + kvh * P.src.head_stride;
-    const long long db = (long long)seq * P.dst.seq_stride + kvh * P.dst.head_stride;
-    for (int i = chunk * (256 / LPR) + sub; i < count; i += P.chunks * (256 / LPR)) {
-        const int from = P.index[(long long)g * P.keep + i];
-        if (in_place && from == i) continue;
-        const long long s = sb + from * P.src.slot_stride + l * 8, d = db + i * P.dst.slot_stride + l * 8;
-        const uint4 a = *reinterpret_cast<const uint4 *>(P.src.k + s), b = *reinterpret_cast<const uint4 *>(P.src.v + s);
-        *reinterpret_cast<uint4 *>(P.dst.k + d) = a;
-        *reinterpret_cast<uint4 *>(P.dst.v + d) = b;
-        if (l == 0) {
-            P.dst.pos[(long long)g * P.dst.cap + i] = P.src.pos[(long long)g * P.src.cap + from];
-            P.dst.acc[(long long)g * P.dst.cap + i] = P.src.acc[(long long)g * P.src.cap + from];
+    const long long sb = (long long)seq * P.src.seq_stride + kvh * P.src.head_stride + l * 8;
+    const long long db = (long long)seq * P.dst.seq_stride + kvh * P.dst.head_stride + l * 8;
+    for (int i0 = chunk * (ROWS * U) + sub; i0 < count; i0 += P.chunks * (ROWS * U)) {
+        int from[U];
+        uint4 a[U], b[U];
+        int p[U];
+        float w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * ROWS;
+            from[u] = i < count ? P.index[(long long)g * P.keep + i] : -1;
+            if (in_place && from[u] == i) from[u] = -1;
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (from[u] >= 0) {
+                a[u] = *reinterpret_cast<const uint4 *>(P.src.k + sb + from[u] * P.src.slot_stride);
+                b[u] = *reinterpret_cast<const uint4 *>(P.src.v + sb + from[u] * P.src.slot_stride);
+                if (l == 0) {
+                    p[u] = P.src.pos[(long long)g * P.src.cap + from[u]];
+                    w[u] = P.src.acc[(long long)g * P.src.cap + from[u]];
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (from[u] >= 0) {
+                const int i = i0 + u * ROWS;
+                *reinterpret_cast<uint4 *>(P.dst.k + db + i * P.dst.slot_stride) = a[u];
+                *reinterpret_cast<uint4 *>(P.dst.v + db + i * P.dst.slot_stride) = b[u];
+                if (l == 0) {
+                    P.dst.pos[(long long)g * P.dst.cap + i] = p[u];
+                    P.dst.acc[(long long)g * P.dst.cap + i] = w[u];
+                }
+            }
     }
 }
 

@@ -355,6 +355,11 @@ def test_evict_long_caches(dev):
     run_evict(2, 1, 1, 64, 130001, [130000], 65000, 4, 128, in_place=True)
 
 
+def test_evict_caches_past_a_cluster(dev):
+    run_evict(1, 1, 2, 64, 262145, [262145], 3000, 4, 128)
+    run_evict(2, 2, 1, 64, 262144, [262144, 5000], 4000, 4, 128, in_place=True)
+
+
 # --------------------------------------------------------------------------- together, and recorded
 def test_a_decode_loop_with_all_three_recorded_as_a_graph(dev):
     """Steps of norm + store, attention with weights and (at the end) an eviction, once call by call and once as a
