@@ -1,5 +1,6 @@
 // Entry points of the attention half of a decode layer: query/key norms with rotation and cache store, attention
 // behind a shared prefix, cache eviction.  Declared in include/peregrine_b200.h.
+#include <cmath>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -75,28 +76,30 @@ int by_type(int D, int dtype, F &&f) {  // f.template operator()<D, BF16>()
     return f.template operator()<256, false>();
 }
 
+template <typename K>
+int opt_in(K kernel, int bytes) {  // per device and cheap: set on every launch that needs it
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    return e == cudaSuccess ? 1 : refuse("shared-memory opt-in: %s", cudaGetErrorString(e));
+}
+
 struct NormRopeLaunch {
     NormRopeArgs &P;
     int S, sms;
     cudaStream_t stream;
     template <int D, bool BF16>
     int operator()() const {
-        // Items of `per` steps of a row are dealt to the warps in rounds; the row's angles cost an item about two steps.
-        const int warps = 2 * kNrWarps * sms, steps = ((P.H + 2 * P.kv.n_kv) * D + 255) / 256;
-        long long best = -1;
-        for (int per = 1; per <= steps; ++per) {
-            const long long items = (long long)S * ((steps + per - 1) / per), cost = (items + warps - 1) / warps * (per + 2);
-            if (best < 0 || cost < best) {
-                best = cost;
-                P.per = per;
-            }
-        }
+        // a warp gets a stretch of items: as long ones as leave none without
+        const int warps = kNrPerSm * kNrWarps * sms, steps = ((P.H + 2 * P.kv.n_kv) * D + 255) / 256;
+        const long long all = (long long)S * steps;
         P.rows = S;
         P.steps = steps;
+        const long long per = (all + warps - 1) / warps;
+        P.per = (int)(per > kNrSteps ? kNrSteps : per);
         P.parts = (steps + P.per - 1) / P.per;
         if ((long long)S * P.parts > 0x7fffffffll) return refuse("pipe_qk_norm_rope: too many rows and heads");
-        const long long need = ((long long)S * P.parts + kNrWarps - 1) / kNrWarps;
-        norm_rope_kernel<D, BF16><<<dim3((unsigned)(need < 2 * sms ? need : 2 * sms)), kNrWarps * 32, 0, stream>>>(P);
+        const long long need = ((long long)S * P.parts + kNrWarps - 1) / kNrWarps, most = (long long)kNrPerSm * sms;
+        if (!opt_in(norm_rope_kernel<D, BF16>, kNrSmem)) return 0;
+        norm_rope_kernel<D, BF16><<<dim3((unsigned)(need < most ? need : most)), kNrWarps * 32, kNrSmem, stream>>>(P);
         return launched("qk_norm_rope launch");
     }
 };
@@ -175,12 +178,6 @@ int kv_map(CUtensorMap *m, const void *p, const KvArgs &kv, int dtype) {
     return enc(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(p), dims, strides,
                box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <typename K>
-int opt_in(K kernel, int bytes) {  // per device and cheap: set on every launch that needs it
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    return e == cudaSuccess ? 1 : refuse("shared-memory opt-in: %s", cudaGetErrorString(e));
 }
 
 // A launch that may start while the one before it in the stream still runs.
@@ -265,10 +262,11 @@ PGB_EXPORT int coli_cuda_pipe_qk_norm_rope(int device, void *q_out, const float 
     P.pos = pos_dev;
     P.base = base_dev;
     P.rows_per_seq = rows_per_seq;
-    P.theta = theta;
+    P.log2_theta = R ? std::log2((double)theta) : 0.0;
     P.R = R;
     P.style = style;
     if (!ctx_of(device, &c)) return refuse("%s: device %d is not initialised", what, device);
+    P.err = c.err;
     DeviceGuard g(c.device);
     if (!g.ok()) return refuse("%s: device %d cannot be selected", what, device);
     return by_type(kv->D, kv->dtype, NormRopeLaunch{P, S, c.sms, c.stream});

@@ -185,6 +185,7 @@ __device__ __forceinline__ int cluster_ld16(const uint16_t *p, int rank) {
 template <int C>
 __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(const EvictArgs P, int part_most) {
     constexpr int W = kEvPartThreads / 32;
+    static_assert(kEvPartThreads >= 256, "a thread per digit");
     extern __shared__ __align__(16) uint32_t ev_key[];
     uint16_t *surv = reinterpret_cast<uint16_t *>(ev_key + part_most);  // the part's kept slots behind `keep`, in order
     __shared__ int s_hist[2][256], s_last, s_ties, s_far, s_holes, s_digit, s_above, s_warp[3][W];
@@ -224,20 +225,33 @@ __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(co
     for (int pass = 0; pass < 4; ++pass) {
         const int shift = 24 - 8 * pass;
         int *hist = s_hist[pass & 1];
-        for (int i0 = warp * 32; i0 < n; i0 += kEvPartThreads) {
-            const int i = i0 + lane;
-            const uint32_t key = i < n ? ev_key[i] : 0u;
-            const bool in = i < n && (pass == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
-            const int digit = in ? (int)((key >> shift) & 255) : -1;
-            const uint32_t same = __match_any_sync(0xffffffffu, digit);  // weights share their leading digits
-            if (in && (same & ((1u << lane) - 1)) == 0) atomicAdd(&hist[digit], __popc(same));
+        for (int i0 = warp * 32; i0 < n; i0 += 4 * kEvPartThreads) {
+            int digit[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + u * kEvPartThreads + lane;
+                const uint32_t key = i < n ? ev_key[i] : 0u;
+                const bool in = i < n && (pass == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
+                digit[u] = in ? (int)((key >> shift) & 255) : -1;
+            }
+            if (pass == 0) {  // weights share their leading digits: one addition for a warp's equal ones
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t same = __match_any_sync(0xffffffffu, digit[u]);
+                    if (digit[u] >= 0 && (same & ((1u << lane) - 1)) == 0) atomicAdd(&hist[digit[u]], __popc(same));
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (digit[u] >= 0) atomicAdd(&hist[digit[u]], 1);
+            }
         }
         cluster_sync<C>();
         int mine = 0;
         if (tid < 256) {
 #pragma unroll
             for (int r = 0; r < C; ++r) mine += cluster_ld<C>(&hist[255 - tid], r);
-            s_hist[(pass + 1) & 1][tid] = 0;  // read by all before the last barrier but one
+            s_hist[(pass + 1) & 1][tid] = 0;  // read by all before this barrier
         }
         int x = mine;
 #pragma unroll
@@ -248,7 +262,8 @@ __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(co
         if (lane == 31) s_warp[0][warp] = x;
         __syncthreads();
         int above = x - mine;  // keys of a larger digit
-        for (int w = 0; w < min(warp, 8); ++w) above += s_warp[0][w];
+#pragma unroll
+        for (int w = 0; w < W; ++w) above += w < warp ? s_warp[0][w] : 0;
         if (tid < 256 && above < want && above + mine >= want) {
             s_digit = 255 - tid;
             s_above = above;
@@ -260,6 +275,7 @@ __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(co
     // Warps own runs of the part: `want` of the slots with this very key are kept, the lowest ones.
     const int run = (n + W * 32 - 1) / (W * 32) * 32, a0 = min(warp * run, n), a1 = min(a0 + run, n);
     int ties = 0;
+#pragma unroll 4
     for (int i = a0 + lane; i < a0 + run; i += 32) ties += i < a1 && ev_key[i] == prefix;
     ties = __reduce_add_sync(0xffffffffu, ties);
     if (lane == 0) {
@@ -272,6 +288,7 @@ __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(co
     for (int w = 0; w < warp; ++w) before += s_warp[0][w];
     const uint32_t below = (1u << lane) - 1;
     int far = 0, holes = 0;
+#pragma unroll 4
     for (int i0 = a0, t = before; i0 < a1; i0 += 32) {
         const int i = i0 + lane;
         const uint32_t key = i < a1 ? ev_key[i] : 0u;
@@ -293,6 +310,7 @@ __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(co
         f += s_warp[1][w];
         h += s_warp[2][w];
     }
+#pragma unroll 4
     for (int i0 = a0, t = before; i0 < a1; i0 += 32) {
         const int i = i0 + lane;
         const uint32_t key = i < a1 ? ev_key[i] : 0u;
