@@ -208,15 +208,18 @@ __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(co
     if (tid < 256) s_hist[0][tid] = s_hist[1][tid] = 0;
     __syncthreads();
     int last = INT_MIN;
-#pragma unroll 4
-    for (int i = tid; i < n; i += kEvPartThreads) last = max(last, pos[i]);
+#pragma unroll 8
+    for (int i = tid; i < n; i += kEvPartThreads) {
+        last = max(last, pos[i]);
+        ev_key[i] = __float_as_uint(acc[i]);
+    }
     last = __reduce_max_sync(0xffffffffu, last);
     if (lane == 0) atomicMax(&s_last, last);
     cluster_sync<C>();
 #pragma unroll
     for (int r = 0; r < C; ++r) last = max(r ? last : INT_MIN, cluster_ld<C>(&s_last, r));
-#pragma unroll 4
-    for (int i = tid; i < n; i += kEvPartThreads) ev_key[i] = evict_key(acc[i], pos[i], last, P.sinks, P.recent);
+#pragma unroll 8
+    for (int i = tid; i < n; i += kEvPartThreads) ev_key[i] = evict_key(__uint_as_float(ev_key[i]), pos[i], last, P.sinks, P.recent);
     __syncthreads();
     // radix select: `prefix` = the digits of the count-th largest key found so far, `want` = its rank among equals
     uint32_t prefix = 0;
@@ -286,18 +289,29 @@ __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(co
     int before = 0;
     for (int r = 0; r < rank; ++r) before += cluster_ld<C>(&s_ties, r);
     for (int w = 0; w < warp; ++w) before += s_warp[0][w];
+    // One word of kept flags for every 32 slots, in the place of their first key.
     const uint32_t below = (1u << lane) - 1;
-    int far = 0, holes = 0;
 #pragma unroll 4
     for (int i0 = a0, t = before; i0 < a1; i0 += 32) {
         const int i = i0 + lane;
         const uint32_t key = i < a1 ? ev_key[i] : 0u;
         const uint32_t tb = __ballot_sync(0xffffffffu, i < a1 && key == prefix);
-        const bool kept = i < a1 && (key > prefix || (key == prefix && t + __popc(tb & below) < want));
+        const uint32_t kept = __ballot_sync(0xffffffffu, i < a1 && (key > prefix || (key == prefix && t + __popc(tb & below) < want)));
         t += __popc(tb);
-        far += __popc(__ballot_sync(0xffffffffu, kept && lo + i >= P.keep));
-        holes += __popc(__ballot_sync(0xffffffffu, i < a1 && !kept && lo + i < P.keep));
+        if (lane == 0) ev_key[i0] = kept;
     }
+    __syncwarp();
+    // of a word: the slots before `keep`, kept ones behind it, free ones before it
+    auto low_of = [&](int i0) { return P.keep - lo - i0 >= 32 ? 0xffffffffu : P.keep - lo - i0 <= 0 ? 0u : (1u << (P.keep - lo - i0)) - 1; };
+    auto in_of = [&](int i0) { return a1 - i0 >= 32 ? 0xffffffffu : (1u << (a1 - i0)) - 1; };
+    int far = 0, holes = 0;
+    for (int i0 = a0 + 32 * lane; i0 < a1; i0 += 1024) {
+        const uint32_t kept = ev_key[i0], low = low_of(i0);
+        far += __popc(kept & ~low);
+        holes += __popc(in_of(i0) & ~kept & low);
+    }
+    far = __reduce_add_sync(0xffffffffu, far);
+    holes = __reduce_add_sync(0xffffffffu, holes);
     if (lane == 0) {
         s_warp[1][warp] = far;
         s_warp[2][warp] = holes;
@@ -311,15 +325,10 @@ __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(co
         h += s_warp[2][w];
     }
 #pragma unroll 4
-    for (int i0 = a0, t = before; i0 < a1; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t key = i < a1 ? ev_key[i] : 0u;
-        const uint32_t tb = __ballot_sync(0xffffffffu, i < a1 && key == prefix);
-        const bool kept = i < a1 && (key > prefix || (key == prefix && t + __popc(tb & below) < want));
-        t += __popc(tb);
-        const uint32_t fb = __ballot_sync(0xffffffffu, kept && lo + i >= P.keep);
-        if (kept && lo + i >= P.keep) surv[f + __popc(fb & below)] = (uint16_t)i;
-        f += __popc(fb);
+    for (int i0 = a0; i0 < a1; i0 += 32) {
+        const uint32_t fk = ev_key[i0] & ~low_of(i0);
+        if ((fk >> lane) & 1u) surv[f + __popc(fk & below)] = (uint16_t)(i0 + lane);
+        f += __popc(fk);
     }
     cluster_sync<C>();
     int fars[C];  // kept slots behind `keep` in the parts before the r-th
@@ -332,25 +341,20 @@ __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(co
             if (r < rank) h += cluster_ld<C>(&s_holes, r);
         }
     }
-    for (int i0 = a0, t = before; i0 < a1 && lo + i0 < P.keep; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t key = i < a1 ? ev_key[i] : 0u;
-        const uint32_t tb = __ballot_sync(0xffffffffu, i < a1 && key == prefix);
-        const bool kept = i < a1 && (key > prefix || (key == prefix && t + __popc(tb & below) < want));
-        t += __popc(tb);
-        const bool hole = i < a1 && !kept && lo + i < P.keep;
-        const uint32_t hb = __ballot_sync(0xffffffffu, hole);
-        if (hole) {
-            const int m = h + __popc(hb & below);
+#pragma unroll 2
+    for (int i0 = a0; i0 < a1 && lo + i0 < P.keep; i0 += 32) {
+        const uint32_t kept = ev_key[i0], low = low_of(i0), hk = in_of(i0) & ~kept & low;
+        if ((hk >> lane) & 1u) {
+            const int m = h + __popc(hk & below);
             int r = 0, first = 0;
 #pragma unroll
             for (int q = 1; q < C; ++q)
                 if (fars[q] <= m) r = q, first = fars[q];
-            index[lo + i] = r * part + cluster_ld16<C>(&surv[m - first], r);
-        } else if (kept && lo + i < P.keep) {
-            index[lo + i] = lo + i;
+            index[lo + i0 + lane] = r * part + cluster_ld16<C>(&surv[m - first], r);
+        } else if ((kept & low) >> lane & 1u) {
+            index[lo + i0 + lane] = lo + i0 + lane;
         }
-        h += __popc(hb);
+        h += __popc(hk);
     }
     cluster_sync<C>();  // nobody leaves while its shared memory is read
 }
