@@ -80,7 +80,10 @@ def verify_drafts(forward_rows: Callable[[np.ndarray], np.ndarray], next_of: Seq
 
 def stack_forward_rows(stack) -> Callable[[np.ndarray], np.ndarray]:
     """``forward_rows`` over a ``DeviceStack``: the rows are one decode step of the resident stack,
-    padded to its batch (the padding rows are computed and dropped)."""
+    padded to its batch (the padding rows are computed and dropped).  The rows do not see each other's
+    history, so a stack with attention layers is refused."""
+    if stack.attn:
+        raise ValueError("verify_drafts: rows of a stack with attention depend on more than their token")
 
     def run(tokens: np.ndarray) -> np.ndarray:
         tokens = np.asarray(tokens, np.int32)

@@ -44,6 +44,20 @@ class SynthLayer:
     shared: SynthExpert | None = None
 
 
+@dataclass
+class SynthAttention:
+    """Grouped-query attention of one layer: merged int4 q/k/v projection, norms per head, output projection."""
+
+    heads: int
+    kv_heads: int
+    head_dim: int
+    norm: np.ndarray    # fp32 [hidden], before the projection
+    wqkv: SynthMatrix   # [(heads + 2 kv_heads) * head_dim, hidden]
+    wo: SynthMatrix     # [hidden, heads * head_dim]
+    q_norm: np.ndarray  # fp32 [head_dim]
+    k_norm: np.ndarray
+
+
 def synth_matrix(rng: np.random.Generator, o_n: int, i_n: int, gs: int, scale_std: float = 0.02) -> SynthMatrix:
     rb = (i_n + 1) // 2
     q = rng.integers(0, 256, size=o_n * rb, dtype=np.uint8)
@@ -58,6 +72,16 @@ def synth_matrix(rng: np.random.Generator, o_n: int, i_n: int, gs: int, scale_st
 def synth_expert(rng, hidden: int, inter: int, gs: int, scale_std: float = 0.02) -> SynthExpert:
     return SynthExpert(synth_matrix(rng, inter, hidden, gs, scale_std), synth_matrix(rng, inter, hidden, gs, scale_std),
                        synth_matrix(rng, hidden, inter, gs, scale_std))
+
+
+def synth_attention(rng, hidden: int, heads: int, kv_heads: int, head_dim: int, gs: int,
+                    scale_std: float = 0.02) -> SynthAttention:
+    def weight(n):
+        return (1.0 + 0.1 * rng.standard_normal(n)).astype(np.float32)
+
+    return SynthAttention(heads, kv_heads, head_dim, weight(hidden),
+                          synth_matrix(rng, (heads + 2 * kv_heads) * head_dim, hidden, gs, scale_std),
+                          synth_matrix(rng, hidden, heads * head_dim, gs, scale_std), weight(head_dim), weight(head_dim))
 
 
 def zipf_bias(rng, n_experts: int, s: float = 1.1, strength: float = 0.35) -> np.ndarray:
