@@ -35,35 +35,43 @@ class KvView:
         self._ref = C.byref(self._c)
 
 
-def _lib():
+_norm = _attend = _workspace = _evict = None  # the library's functions, bound at the first call
+
+
+def _bind():
+    global _norm, _attend, _workspace, _evict
     L = cuda.lib()
-    if L.coli_cuda_pipe_attention.argtypes is None:
-        vp, i, f, ll, sz = C.c_void_p, C.c_int, C.c_float, C.c_longlong, C.c_size_t
-        L.coli_cuda_pipe_qk_norm_rope.argtypes = [i, vp, vp, ll, i, i, vp, vp, vp, f, vp, vp, i, f, i, i]
-        L.coli_cuda_pipe_attention_workspace.argtypes = [i, i, i, vp, i, i]
-        L.coli_cuda_pipe_attention_workspace.restype = sz
-        L.coli_cuda_pipe_kv_evict.argtypes = [i, vp, vp, vp, vp, vp, i, i, i]
-        L.coli_cuda_pipe_attention.argtypes = [i, vp, i, vp, i, i, vp, i, vp, vp, i, vp, f, vp, sz]
-    return L
+    vp, i, f, ll, sz = C.c_void_p, C.c_int, C.c_float, C.c_longlong, C.c_size_t
+    _norm, _attend = L.coli_cuda_pipe_qk_norm_rope, L.coli_cuda_pipe_attention
+    _workspace, _evict = L.coli_cuda_pipe_attention_workspace, L.coli_cuda_pipe_kv_evict
+    _norm.argtypes = [i, vp, vp, ll, i, i, vp, vp, vp, f, vp, vp, i, f, i, i]
+    _workspace.argtypes = [i, i, i, vp, i, i]
+    _workspace.restype = sz
+    _evict.argtypes = [i, vp, vp, vp, vp, vp, i, i, i]
+    _attend.argtypes = [i, vp, i, vp, i, i, vp, i, vp, vp, i, vp, f, vp, sz]
 
 
 def qk_norm_rope(device: int, q_out: int, qkv: int, rows: int, heads: int, kv: KvView, base: int, pos: int,
                  theta: float, rotary: int | None = None, style: int = 0, q_weight: int = 0, k_weight: int = 0,
                  eps: float = 1e-6, rows_per_seq: int = 1, row_stride: int | None = None) -> None:
     """Rows of a merged q/k/v projection -> normed, rotated queries in ``q_out`` and keys and values in the cache."""
+    if _norm is None:
+        _bind()
     if rotary is None:
         rotary = kv.head_dim
     if row_stride is None:
         row_stride = (heads + 2 * kv.n_kv) * kv.head_dim
-    if _lib().coli_cuda_pipe_qk_norm_rope(device, q_out, qkv, row_stride, rows, heads, kv._ref, q_weight or None,
-                                          k_weight or None, eps, pos, base, rows_per_seq, theta, rotary, style) != 1:
+    if _norm(device, q_out, qkv, row_stride, rows, heads, kv._ref, q_weight, k_weight, eps, pos, base, rows_per_seq,
+             theta, rotary, style) != 1:
         raise cuda.CudaError("cuda pipe_qk_norm_rope failed")
 
 
 def attention_workspace(device: int, rows: int, heads: int, own: KvView, prefix_len: int = 0,
                         rows_per_seq: int = 1) -> int:
     """Bytes of scratch that ``attention`` needs for calls of this shape."""
-    n = _lib().coli_cuda_pipe_attention_workspace(device, rows, heads, own._ref, prefix_len, rows_per_seq)
+    if _workspace is None:
+        _bind()
+    n = _workspace(device, rows, heads, own._ref, prefix_len, rows_per_seq)
     if n == 0:
         raise cuda.CudaError("cuda pipe_attention_workspace: shape refused")
     return int(n)
@@ -73,15 +81,17 @@ def attention(device: int, out: int, q: int, rows: int, heads: int, own: KvView,
               work_bytes: int, rows_per_seq: int = 1, prefix: KvView | None = None, prefix_len: int = 0, mask: int = 0,
               out_f32: bool = True) -> None:
     """Attention of every sequence over the shared prefix and its own slots; adds to ``own``'s acc when it has one."""
-    if _lib().coli_cuda_pipe_attention(device, out, 1 if out_f32 else 0, q, rows, heads,
-                                       None if prefix is None else prefix._ref, prefix_len, own._ref, base,
-                                       rows_per_seq, mask or None, scale, work, work_bytes) != 1:
+    if _attend is None:
+        _bind()
+    if _attend(device, out, 1 if out_f32 else 0, q, rows, heads, None if prefix is None else prefix._ref, prefix_len,
+               own._ref, base, rows_per_seq, mask, scale, work, work_bytes) != 1:
         raise cuda.CudaError("cuda pipe_attention failed")
 
 
 def kv_evict(device: int, dst: KvView, src: KvView, length: int, new_length: int, index: int, keep: int,
              sinks: int = 0, recent: int = 0) -> None:
     """Keeps the ``keep`` best slots of every sequence and head (``dst`` may be ``src``)."""
-    if _lib().coli_cuda_pipe_kv_evict(device, dst._ref, src._ref, length, new_length, index, keep, sinks,
-                                      recent) != 1:
+    if _evict is None:
+        _bind()
+    if _evict(device, dst._ref, src._ref, length, new_length, index, keep, sinks, recent) != 1:
         raise cuda.CudaError("cuda pipe_kv_evict failed")

@@ -4,6 +4,8 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <mutex>
+#include <vector>
 
 #include "../../include/peregrine_b200.h"
 #include "ctx.h"
@@ -76,10 +78,56 @@ int by_type(int D, int dtype, F &&f) {  // f.template operator()<D, BF16>()
     return f.template operator()<256, false>();
 }
 
+// Dynamic shared-memory opt-in, once per kernel and device (cudaFuncSetAttribute takes a microsecond of every call otherwise).
+struct OptIn {
+    const void *fn;
+    int device, bytes;
+};
+std::mutex g_opt_mu;
+std::vector<OptIn> g_opt;
+
 template <typename K>
-int opt_in(K kernel, int bytes) {  // per device and cheap: set on every launch that needs it
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    return e == cudaSuccess ? 1 : refuse("shared-memory opt-in: %s", cudaGetErrorString(e));
+int opt_in(K kernel, int bytes) {
+    const void *fn = reinterpret_cast<const void *>(kernel);
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return refuse("shared-memory opt-in: no current device");
+    std::lock_guard<std::mutex> lk(g_opt_mu);
+    for (OptIn &e : g_opt)
+        if (e.fn == fn && e.device == device) {
+            if (e.bytes >= bytes) return 1;
+            const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (r == cudaSuccess) e.bytes = bytes;
+            return r == cudaSuccess ? 1 : refuse("shared-memory opt-in: %s", cudaGetErrorString(r));
+        }
+    const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (r != cudaSuccess) return refuse("shared-memory opt-in: %s", cudaGetErrorString(r));
+    g_opt.push_back({fn, device, bytes});
+    return 1;
+}
+
+// A launch that may start while the one before it in the stream still runs: every kernel here sets itself up, waits on the
+// device for what came before (the one launch that need not says so), and only then lets the next one start.  `early` false:
+// an ordinary launch.  A grid that fills the device is placed unevenly while the one before still holds some SMs: six
+// sequences' eviction took 59 us early and 52 in order, a split of two long sequences 83 and 70; a call of one sequence 9.5
+// early and 12.3 in order.
+template <typename... K, typename... A>
+int launch_early(void (*kernel)(K...), unsigned grid, int block, int smem, cudaStream_t stream, const char *what, int cluster, bool early,
+                 A... args) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = early;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3((unsigned)block);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, K(args)...);
+    return launched(what);
 }
 
 struct NormRopeLaunch {
@@ -99,8 +147,8 @@ struct NormRopeLaunch {
         if ((long long)S * P.parts > 0x7fffffffll) return refuse("pipe_qk_norm_rope: too many rows and heads");
         const long long need = ((long long)S * P.parts + kNrWarps - 1) / kNrWarps, most = (long long)kNrPerSm * sms;
         if (!opt_in(norm_rope_kernel<D, BF16>, kNrSmem)) return 0;
-        norm_rope_kernel<D, BF16><<<dim3((unsigned)(need < most ? need : most)), kNrWarps * 32, kNrSmem, stream>>>(P);
-        return launched("qk_norm_rope launch");
+        return launch_early(norm_rope_kernel<D, BF16>, (unsigned)(need < most ? need : most), kNrWarps * 32, kNrSmem, stream,
+                            "qk_norm_rope launch", 1, true, P);
     }
 };
 
@@ -180,23 +228,6 @@ int kv_map(CUtensorMap *m, const void *p, const KvArgs &kv, int dtype) {
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A launch that may start while the one before it in the stream still runs.
-template <typename... K, typename... A>
-int launch_early(void (*kernel)(K...), unsigned grid, int block, int smem, cudaStream_t stream, const char *what, A... args) {
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3((unsigned)block);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, K(args)...);
-    return launched(what);
-}
-
 struct AttnLaunch {
     const AttnArgs &P;
     const CUtensorMap *maps;  // of the prefix's and the own keys and values
@@ -211,21 +242,21 @@ struct AttnLaunch {
             static_assert(T::ROWS == (D == 256 ? 128 : 256), "as planned");
             auto tc = attn_tc_kernel<D, BF16, F32>;
             if (!opt_in(tc, T::SMEM)) return 0;
-            tc<<<dim3(P.tc_ctas), T::THREADS, T::SMEM, stream>>>(P, maps[0], maps[1], maps[2], maps[3]);
-            if (!launched("attention tensor launch")) return 0;
-            // needs nothing of the one before: it fills the SMs that this leaves, and ends after it
-            if (!launch_early(split, P.ctas, kAtThreads, kSmem, stream, "attention launch", P, maps[0], maps[1], maps[2], maps[3])) return 0;
-        } else {
-            split<<<dim3(P.ctas), kAtThreads, kSmem, stream>>>(P, maps[0], maps[1], maps[2], maps[3]);
-            if (!launched("attention launch")) return 0;
+            if (!launch_early(tc, P.tc_ctas, T::THREADS, T::SMEM, stream, "attention tensor launch", 1, true, P, maps[0], maps[1], maps[2], maps[3]))
+                return 0;
         }
+        // (behind the tensor-memory kernel it fills the SMs that this leaves, and ends after it)
+        const long long tiles = (long long)P.own.n_kv * ((long long)P.own.n_seq * P.mt_own * (P.own.cap / kAtKeys + 1) +
+                                                         (long long)P.mt_pre * (P.prefix_len / kAtKeys + 1));  // at the most
+        const bool early = P.tc_pre || P.tc_own || tiles <= 2 * P.ctas;
+        if (!launch_early(split, P.ctas, kAtThreads, kSmem, stream, "attention launch", 1, early, P, maps[0], maps[1], maps[2], maps[3])) return 0;
         // waits on the device for the end of the launches before
         const long long vectors = (long long)P.S * P.H, chunks = P.own.acc ? (P.own.cap + kAtChunk - 1) / kAtChunk : 0;
         const bool few = vectors < 4 * P.tc_ctas;
         const int row_ctas = (int)(few ? vectors : (vectors + 3) / 4);
         const unsigned grid = (unsigned)(row_ctas + chunks * P.own.n_seq * P.own.n_kv);
         return launch_early(few ? attn_join_kernel<D, BF16, 4> : attn_join_kernel<D, BF16, 1>, grid, kAtCombine, 0, stream,
-                            "attention join launch", P, RT, row_ctas, (int)chunks);
+                            "attention join launch", 1, true, P, RT, row_ctas, (int)chunks);
     }
     template <int D, bool BF16>
     int operator()() const {
@@ -235,6 +266,11 @@ struct AttnLaunch {
 };
 
 }  // namespace
+
+void pgb::forget_opt_ins() {
+    std::lock_guard<std::mutex> lk(g_opt_mu);
+    g_opt.clear();
+}
 
 PGB_EXPORT int coli_cuda_pipe_qk_norm_rope(int device, void *q_out, const float *qkv_dev, long long row_stride, int S,
                                            int H, const ColiCudaKv *kv, const float *q_w, const float *k_w, float eps,
@@ -368,29 +404,17 @@ PGB_EXPORT int coli_cuda_pipe_kv_evict(int device, const ColiCudaKv *dst, const 
     DeviceGuard g(c.device);
     if (!g.ok()) return refuse("%s: device %d cannot be selected", what, device);
     if (src->cap > kEvCluster * kEvPartMost) {
-        evict_select_kernel<<<dim3((unsigned)groups), kEvThreads, 0, c.stream>>>(P);
-        if (!launched("kv_evict select launch")) return 0;
+        if (!launch_early(evict_select_kernel, (unsigned)groups, kEvThreads, 0, c.stream, "kv_evict select launch", 1, false, P)) return 0;
     } else {
         const int parts = src->cap <= kEvAlone ? 1 : kEvCluster, most = (((src->cap + parts - 1) / parts) + 7) & ~7, smem = most * 6;
         auto kernel = parts == 1 ? evict_select_cluster_kernel<1> : evict_select_cluster_kernel<kEvCluster>;
         if (!opt_in(kernel, smem)) return 0;
-        cudaLaunchConfig_t cfg{};
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)parts;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.gridDim = dim3((unsigned)(groups * parts));
-        cfg.blockDim = dim3(kEvPartThreads);
-        cfg.dynamicSmemBytes = (size_t)smem;
-        cfg.stream = c.stream;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        cudaLaunchKernelEx(&cfg, kernel, (const EvictArgs)P, most);
-        if (!launched("kv_evict select launch")) return 0;
+        if (!launch_early(kernel, (unsigned)(groups * parts), kEvPartThreads, smem, c.stream, "kv_evict select launch", parts, groups * parts <= c.sms, P, most))
+            return 0;
     }
     const int per_cta = 4 * 256 / (src->D / 8);
     const long long most = ((long long)keep + per_cta - 1) / per_cta, want = (16ll * c.sms + groups - 1) / groups;
     P.chunks = (int)(most < want ? most : want);
     auto move = src->D == 64 ? evict_move_kernel<64> : src->D == 128 ? evict_move_kernel<128> : evict_move_kernel<256>;
-    return launch_early(move, (unsigned)(groups * P.chunks), 256, 0, c.stream, "kv_evict move launch", P);
+    return launch_early(move, (unsigned)(groups * P.chunks), 256, 0, c.stream, "kv_evict move launch", 1, true, P);
 }

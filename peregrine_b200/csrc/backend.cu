@@ -273,6 +273,7 @@ PGB_EXPORT void coli_cuda_shutdown(void) {
         std::lock_guard<std::mutex> lk(g_smem_mu);
         g_smem_optin[i].clear();
     }
+    pgb::forget_opt_ins();
     g_nctx = 0;
     t_current_device = -1;
 }

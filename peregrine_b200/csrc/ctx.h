@@ -12,6 +12,7 @@ struct CtxRef {
 
 int ctx_of(int device, CtxRef *ref);  // 0 when the device was not initialised
 void count_launches(int n);
+void forget_opt_ins();  // attn.cu: kernel attributes are set anew (at shutdown)
 
 // Makes a context's device current for one call and puts the caller's back.
 class DeviceGuard {

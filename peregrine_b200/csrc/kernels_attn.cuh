@@ -441,7 +441,6 @@ __global__ void __launch_bounds__(kAtThreads, SplitShape<D, RT>::PER_SM)
     __shared__ __align__(8) unsigned long long s_bar[2 * NS];
     __shared__ int s_fail;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
-    griddep_launch_dependents();
     const uint32_t full = smem_u32(s_bar), empty = full + 8 * NS;
     volatile int *fail = &s_fail;
     if (tid == 128) {
@@ -452,6 +451,10 @@ __global__ void __launch_bounds__(kAtThreads, SplitShape<D, RT>::PER_SM)
         }
         fence_mbar_init();
     }
+    // The tensor-memory kernel before this one lets it begin when all before itself is done: nothing to wait for then.
+    const bool alone = !P.tc_pre && !P.tc_own;
+    if (alone) griddep_wait();
+    griddep_launch_dependents();
     const int nkv = P.own.n_kv, per_seq = nkv * P.mt_own;
     const int tp = P.mt_pre ? (P.prefix_len - P.cut_pre + kAtKeys - 1) / kAtKeys : 0;
     const long long line_pre = (long long)nkv * P.mt_pre * tp;
@@ -703,6 +706,7 @@ template <int D, bool BF16, int WPR>
 __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P, int rt, int row_ctas, int chunks) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     griddep_wait();
+    griddep_launch_dependents();
     if (blockIdx.x < (unsigned)row_ctas) {
         constexpr int E = D / 32;
         __shared__ float s_o[WPR][WPR == 1 ? 1 : D];

@@ -148,7 +148,6 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     __shared__ float s_top[2][T::TILES][2][128];  // a row's two maxima, by turns
     __shared__ int s_fail;
     const int tid = threadIdx.x, warp = tid >> 5, c = blockIdx.x;
-    griddep_launch_dependents();
     uint8_t *base = tc_smem_raw + ((1024 - (smem_u32(tc_smem_raw) & 1023)) & 1023);
     const uint32_t q_s = smem_u32(base), ring_s = q_s + T::TILES * T::Q_BYTES;
     const uint32_t full = smem_u32(s_bar), empty = full + 8 * T::SLOTS, qfull = empty + 8 * T::SLOTS, odone = qfull + 8 * T::TILES,
@@ -178,6 +177,8 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = s_tmem;
+    griddep_wait();
+    griddep_launch_dependents();  // (now, when all before this launch is done: the next one does not wait for it)
     const int nkv = P.own.n_kv, per_seq = nkv * P.tcm_own, tp = P.tc_pre ? P.cut_pre / N + kTcEmpty : 0;
     const long long line_pre = (long long)nkv * P.tcm_pre * tp;
     long long first = 0, end = 0;

@@ -59,6 +59,8 @@ __device__ __forceinline__ int block_scan(int v, int *s_warp, int &total) {
 __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArgs P) {
     __shared__ int s_warp[32], s_hist[256], s_digit, s_above, s_last;
     const int seq = blockIdx.x / P.src.n_kv;
+    griddep_wait();
+    griddep_launch_dependents();
     int len = P.len[seq];
     if (len < 0) return;
     len = min(len, P.src.cap);
@@ -190,6 +192,7 @@ __global__ void __launch_bounds__(kEvPartThreads) evict_select_cluster_kernel(co
     uint16_t *surv = reinterpret_cast<uint16_t *>(ev_key + part_most);  // the part's kept slots behind `keep`, in order
     __shared__ int s_hist[2][256], s_last, s_ties, s_far, s_holes, s_digit, s_above, s_warp[3][W];
     const int rank = C == 1 ? 0 : blockIdx.x % C, g = blockIdx.x / C, seq = g / P.src.n_kv;
+    griddep_wait();
     griddep_launch_dependents();
     int len = P.len[seq];
     if (len < 0) return;
@@ -365,6 +368,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs P) {
     constexpr int LPR = D / 8, ROWS = 256 / LPR, U = 4;
     const int g = blockIdx.x / P.chunks, chunk = blockIdx.x % P.chunks, seq = g / P.src.n_kv, kvh = g % P.src.n_kv;
     griddep_wait();
+    griddep_launch_dependents();
     const int len = P.len[seq];
     const int count = min(min(len, P.src.cap), P.keep);
     if (kvh == 0 && chunk == 0 && threadIdx.x == 0) P.new_len[seq] = min(len, P.keep);

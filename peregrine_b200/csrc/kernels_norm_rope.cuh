@@ -86,9 +86,11 @@ __global__ void __launch_bounds__(kNrWarps * 32, kNrPerSm) norm_rope_kernel(cons
             bulk_g2s(smem_u32(buf + at * kNrSteps * 256), P.qkv + (long long)row * P.row_stride + (long long)h0 * D, (uint32_t)(n * D * 4), bar + 8 * at);
         }
     };
-    if (first < end) fetch(first);
     for (int j = threadIdx.x; j < half; j += blockDim.x)  // turns per position
         s_freq[j] = exp2(-2.0 * j / P.R * P.log2_theta) * 0.15915494309189533577;
+    griddep_wait();
+    griddep_launch_dependents();
+    if (first < end) fetch(first);
     const int sub = lane / LPH, l = lane % LPH, p0 = 4 * l;  // this lane's pairs of a head: p0 .. p0 + 3
     // 16-byte accesses of either pairing need the rotated part to end on a lane's boundary
     const bool wide = (P.R & 7) == 0, turned = p0 < half;
