@@ -169,42 +169,42 @@ size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, i
     const long long m_own = (long long)rows * (H / own.n_kv), m_pre = (long long)S * (H / own.n_kv);
     P->G = H / own.n_kv;
     const int rt = row_tile(rows, H, own.n_kv);
-    const long long mt_own = (m_own + rt - 1) / rt, mt_pre = prefix_len ? (m_pre + rt - 1) / rt : 0;
+    P->tc_pre = prefix_len && m_pre > kTcRows;
+    P->tc_own = m_own > kTcRows;
+    const long long mt_own = P->tc_own ? 0 : (m_own + rt - 1) / rt, mt_pre = prefix_len && !P->tc_pre ? (m_pre + rt - 1) / rt : 0;
     const long long units = own.n_kv * (mt_pre + own.n_seq * mt_own);
-    // tiles of 64 keys of a line are counted in 32 bits per sequence
-    if (units > 0x3fffffff || m_pre > 0x3fffffff || ((long long)own.cap / 64 + 1) * own.n_kv * mt_own > 0x3fffffff) return 0;
-    P->mt_own = (int)mt_own;
-    P->mt_pre = (int)mt_pre;
-    P->ctas = attn_ctas(own.D, rt, sms);
     P->tc_rows = own.D == 256 ? 128 : 256;
     P->tc_ctas = sms;
-    P->tc_pre = m_pre > kTcRows && prefix_len >= kTcKeys;
-    P->tc_own = m_own > kTcRows && own.cap >= kTcKeys;
-    P->cut_pre = P->tc_pre ? prefix_len / kTcKeys * kTcKeys : 0;
     P->tc2_pre = own.D < 256 && m_pre <= 128;
     P->tc2_own = own.D < 256 && m_own <= 128;
-    P->tcm_pre = P->tc_pre ? (int)((m_pre + P->tc_rows - 1) / P->tc_rows) : 0;
-    P->tcm_own = P->tc_own ? (int)((m_own + P->tc_rows - 1) / P->tc_rows) : 0;
+    const long long tcm_pre = P->tc_pre ? (m_pre + P->tc_rows - 1) / P->tc_rows : 0, tcm_own = P->tc_own ? (m_own + P->tc_rows - 1) / P->tc_rows : 0;
+    const long long tc_units = own.n_kv * (tcm_pre + own.n_seq * tcm_own), tiles = (long long)own.cap / 64 + 16;
+    // units and the tiles of one sequence are counted in 32 bits
+    if (units > 0x3fffffff || tc_units > 0x3fffffff || m_pre > 0x3fffffff || tiles * own.n_kv * (mt_own > tcm_own ? mt_own : tcm_own) > 0x3fffffff)
+        return 0;
+    P->mt_own = (int)mt_own;
+    P->mt_pre = (int)mt_pre;
+    P->tcm_pre = (int)tcm_pre;
+    P->tcm_own = (int)tcm_own;
+    P->ctas = units ? attn_ctas(own.D, rt, sms) : 0;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         char *p = work ? work + at : nullptr;
         at += (bytes + 255) & ~(size_t)255;
         return p;
     };
-    const bool tc = P->tc_pre || P->tc_own;
-    const size_t tc_units = tc ? own.n_kv * (P->tcm_pre + (size_t)own.n_seq * P->tcm_own) : 0;
-    const size_t split_rows = ((size_t)units + P->ctas) * rt, tc_rows = tc ? (tc_units + P->tc_ctas) * P->tc_rows : 0;
+    const size_t split_rows = ((size_t)units + P->ctas) * rt, tc_rows = tc_units ? ((size_t)tc_units + P->tc_ctas) * P->tc_rows : 0;
     P->tc_row0 = (long long)split_rows;
     P->part = reinterpret_cast<float *>(take((split_rows + tc_rows) * own.D * 4));
     P->ml = reinterpret_cast<float2 *>(take((split_rows + tc_rows) * 8));
     P->cta_of = reinterpret_cast<int2 *>(take((size_t)units * 8));
-    P->tc_cta_of = reinterpret_cast<int2 *>(take(tc_units * 8));
+    P->tc_cta_of = reinterpret_cast<int2 *>(take((size_t)tc_units * 8));
     P->scores = own.acc ? reinterpret_cast<float *>(take((size_t)own.n_seq * own.n_kv * m_own * own.cap * 4)) : nullptr;
     return at;
 }
 
-// Copies of [keys][64 dims] boxes of a cache, swizzled by 128 bytes.
-int kv_map(CUtensorMap *m, const void *p, const KvArgs &kv, int dtype) {
+// Copies of [64 keys][64 dims] boxes of a cache, swizzled by 128 bytes; slots from `slots` on come as zeros.
+int kv_map(CUtensorMap *m, const void *p, const KvArgs &kv, int slots, int dtype) {
     typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -220,7 +220,7 @@ int kv_map(CUtensorMap *m, const void *p, const KvArgs &kv, int dtype) {
     if (!enc) return 0;
     // a stride of a dimension with one entry is never used, but has to be a valid one
     const long long head = kv.n_kv > 1 ? kv.head_stride : kv.slot_stride, seq = kv.n_seq > 1 ? kv.seq_stride : kv.slot_stride;
-    const cuuint64_t dims[4] = {(cuuint64_t)kv.D, (cuuint64_t)kv.cap, (cuuint64_t)kv.n_kv, (cuuint64_t)kv.n_seq};
+    const cuuint64_t dims[4] = {(cuuint64_t)kv.D, (cuuint64_t)slots, (cuuint64_t)kv.n_kv, (cuuint64_t)kv.n_seq};
     const cuuint64_t strides[3] = {(cuuint64_t)kv.slot_stride * 2, (cuuint64_t)head * 2, (cuuint64_t)seq * 2};
     const cuuint32_t box[4] = {64, kAtKeys, 1, 1}, es[4] = {1, 1, 1, 1};
     return enc(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(p), dims, strides,
@@ -236,7 +236,7 @@ struct AttnLaunch {
     int run() const {
         constexpr int kSmem = SplitShape<D, RT>::SMEM;
         auto split = attn_split_kernel<D, BF16, F32, RT>;
-        if (!opt_in(split, kSmem)) return 0;
+        if (P.ctas && !opt_in(split, kSmem)) return 0;
         if (P.tc_pre || P.tc_own) {
             using T = TcShape<D, BF16, F32>;
             static_assert(T::ROWS == (D == 256 ? 128 : 256), "as planned");
@@ -245,11 +245,13 @@ struct AttnLaunch {
             if (!launch_early(tc, P.tc_ctas, T::THREADS, T::SMEM, stream, "attention tensor launch", 1, true, P, maps[0], maps[1], maps[2], maps[3]))
                 return 0;
         }
-        // (behind the tensor-memory kernel it fills the SMs that this leaves, and ends after it)
-        const long long tiles = (long long)P.own.n_kv * ((long long)P.own.n_seq * P.mt_own * (P.own.cap / kAtKeys + 1) +
-                                                         (long long)P.mt_pre * (P.prefix_len / kAtKeys + 1));  // at the most
-        const bool early = P.tc_pre || P.tc_own || tiles <= 2 * P.ctas;
-        if (!launch_early(split, P.ctas, kAtThreads, kSmem, stream, "attention launch", 1, early, P, maps[0], maps[1], maps[2], maps[3])) return 0;
+        if (P.ctas) {  // (behind the tensor-memory kernel it fills the SMs that this leaves, and ends after it)
+            const long long tiles = (long long)P.own.n_kv * ((long long)P.own.n_seq * P.mt_own * (P.own.cap / kAtKeys + 1) +
+                                                             (long long)P.mt_pre * (P.prefix_len / kAtKeys + 1));  // at the most
+            const bool early = P.tc_pre || tiles <= 2 * P.ctas;
+            if (!launch_early(split, P.ctas, kAtThreads, kSmem, stream, "attention launch", 1, early, P, maps[0], maps[1], maps[2], maps[3]))
+                return 0;
+        }
         // waits on the device for the end of the launches before
         const long long vectors = (long long)P.S * P.H, chunks = P.own.acc ? (P.own.cap + kAtChunk - 1) / kAtChunk : 0;
         const bool few = vectors < 4 * P.tc_ctas;
@@ -364,8 +366,8 @@ PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, 
     if (!g.ok()) return refuse("%s: device %d cannot be selected", what, device);
     CUtensorMap maps[4] = {};
     const int type = own->dtype;
-    if ((prefix_len && !(kv_map(&maps[0], P.pre.k, P.pre, type) && kv_map(&maps[1], P.pre.v, P.pre, type))) ||
-        !(kv_map(&maps[2], P.own.k, P.own, type) && kv_map(&maps[3], P.own.v, P.own, type)))
+    if ((prefix_len && !(kv_map(&maps[0], P.pre.k, P.pre, prefix_len, type) && kv_map(&maps[1], P.pre.v, P.pre, prefix_len, type))) ||
+        !(kv_map(&maps[2], P.own.k, P.own, P.own.cap, type) && kv_map(&maps[3], P.own.v, P.own, P.own.cap, type)))
         return refuse("%s: the cache cannot be described to the copy engine", what);
     if (!prefix_len) {  // not used
         maps[0] = maps[2];

@@ -2,8 +2,7 @@
 //
 // Problems: the prefix, once per kv head, with the rows of ALL sequences (its keys are read once for the batch), and every
 // sequence's own slots per kv head with that sequence's rows.  A problem has M = rows x group query vectors.  Where M is
-// large, its tiles of keys that every row sees go to the tensor-memory kernel (kernels_attn_tc.cuh); this kernel takes
-// the rest in row tiles of 8 or 16.  Work is counted in tiles of 64 keys; all tiles of all problems form one line, and CTA c of
+// large it goes to the tensor-memory kernel (kernels_attn_tc.cuh); this kernel takes the others in row tiles of 8 or 16.  Work is counted in tiles of 64 keys; all tiles of all problems form one line, and CTA c of
 // n takes the c-th equal part of it, whatever the lengths (read on the device): no sequence is too long or too short.  Within its part
 // a CTA keeps the running maximum m, sum l and output of one problem at a time (log2 units)
 //     m' = max(m, x),  l' = l 2^(m-m') + sum 2^(x-m'),  o' = o 2^(m-m') + sum 2^(x-m') v,   x = scale log2(e) q.k
@@ -38,9 +37,8 @@ struct AttnArgs {
     float scale2;                // scale * log2(e)
     int ctas;                    // CTAs that share the line of tiles
     int mt_pre, mt_own;          // row tiles of a problem (mt_pre 0: no prefix)
-    // the tensor-memory kernel: tiles of 64 keys that every row of a problem sees
-    int tc_pre, tc_own;    // whether it takes such tiles of the prefix, of the own slots
-    int cut_pre;           // keys of the prefix that it takes
+    // the tensor-memory kernel
+    int tc_pre, tc_own;    // whether it takes the prefix, the own slots
     int tc_ctas, tc_rows;  // its CTAs, rows of one of its partials
     int tcm_pre, tcm_own;  // its row tiles of a problem
     int tc2_pre, tc2_own;  // 1: a row tile has 128 rows and its keys go to two halves of a partial in turn
@@ -68,12 +66,6 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ int own_keys(const AttnArgs &P, int b) {
     const int base = P.base[b];
     return base < 0 ? 0 : (int)min((long long)base + P.rows, (long long)P.own.cap);
-}
-// How many of them the tensor-memory kernel takes.
-__device__ __forceinline__ int own_cut(const AttnArgs &P, int b) {
-    if (!P.tc_own) return 0;
-    const int base = P.base[b];
-    return base < 0 ? 0 : min(base, P.own.cap) / kTcKeys * kTcKeys;
 }
 // New slots that row i of a sequence sees, a bit each.
 __device__ __forceinline__ unsigned long long row_mask(const AttnArgs &P, int row, int i) {
@@ -130,11 +122,9 @@ __device__ __forceinline__ uint32_t finite16(uint32_t v) {
 
 // A place on the line of tiles: tile `tile` of the row tile `mt` of kv head `kvh` of sequence `seq` (-1: the prefix).
 struct AttnAt {
-    int seq, kvh, mt, tile, tiles, k0, keys, base;  // tile t holds the keys [k0 + 64 t, ...) below `keys`
+    int seq, kvh, mt, tile, tiles, keys, base;  // tile t holds the keys [64 t, ...) below `keys`
 };
-__device__ __forceinline__ int own_tiles(const AttnArgs &P, int b) {
-    return (own_keys(P, b) - own_cut(P, b) + kAtKeys - 1) / kAtKeys;
-}
+__device__ __forceinline__ int own_tiles(const AttnArgs &P, int b) { return P.tc_own ? 0 : (own_keys(P, b) + kAtKeys - 1) / kAtKeys; }
 __device__ __forceinline__ void attn_step(const AttnArgs &P, AttnAt &a) {
     if (++a.tile < a.tiles) return;
     a.tile = 0;
@@ -149,8 +139,7 @@ __device__ __forceinline__ void attn_step(const AttnArgs &P, AttnAt &a) {
         }
         a.base = P.base[a.seq];
         a.keys = own_keys(P, a.seq);
-        a.k0 = own_cut(P, a.seq);
-        a.tiles = (a.keys - a.k0 + kAtKeys - 1) / kAtKeys;
+        a.tiles = own_tiles(P, a.seq);
     } while (a.tiles == 0);
 }
 // Number of the (problem, row tile) on the line.
@@ -264,7 +253,7 @@ __device__ __forceinline__ void attn_tile(const AttnArgs &P, const AttnAt &a, At
 #pragma unroll
             for (int e = 0; e < 2 * J; ++e) s[n][e] = (s[n][e] + s2[n][e]) * P.scale2;
     }
-    const int t0 = a.k0 + a.tile * kAtKeys + kw, col = (lane & 3) * 2;
+    const int t0 = a.tile * kAtKeys + kw, col = (lane & 3) * 2;
     const bool open = t0 + 16 <= min(a.base, a.keys);  // every row sees every key of the range
     uint32_t seen = 0;  // bit 4 n + e: whether s[n][e]'s row sees its key
     if (!open) {
@@ -456,7 +445,7 @@ __global__ void __launch_bounds__(kAtThreads, SplitShape<D, RT>::PER_SM)
     if (alone) griddep_wait();
     griddep_launch_dependents();
     const int nkv = P.own.n_kv, per_seq = nkv * P.mt_own;
-    const int tp = P.mt_pre ? (P.prefix_len - P.cut_pre + kAtKeys - 1) / kAtKeys : 0;
+    const int tp = P.mt_pre ? (P.prefix_len + kAtKeys - 1) / kAtKeys : 0;
     const long long line_pre = (long long)nkv * P.mt_pre * tp;
     long long first, end;
     int seq = 0, off = 0;
@@ -468,7 +457,6 @@ __global__ void __launch_bounds__(kAtThreads, SplitShape<D, RT>::PER_SM)
     if (first < line_pre) {
         at.seq = -1;
         at.base = at.keys = P.prefix_len;
-        at.k0 = P.cut_pre;
         at.tiles = tp;
         const int u = (int)(first / tp);
         at.kvh = u / P.mt_pre;
@@ -478,7 +466,6 @@ __global__ void __launch_bounds__(kAtThreads, SplitShape<D, RT>::PER_SM)
         at.seq = seq;
         at.base = P.base[seq];
         at.keys = own_keys(P, seq);
-        at.k0 = own_cut(P, seq);
         at.tiles = own_tiles(P, seq);
         const int in = (int)(first - line_pre - (long long)off * per_seq);
         const int u = in / at.tiles;
@@ -499,7 +486,7 @@ __global__ void __launch_bounds__(kAtThreads, SplitShape<D, RT>::PER_SM)
                 if (*fail) break;
                 mbar_expect_tx(full + 8 * st, 2 * TB);
                 const CUtensorMap *mk = at.seq < 0 ? &pre_k : &own_k, *mv = at.seq < 0 ? &pre_v : &own_v;
-                const int t0 = at.k0 + at.tile * kAtKeys, sq = at.seq < 0 ? 0 : at.seq;
+                const int t0 = at.tile * kAtKeys, sq = at.seq < 0 ? 0 : at.seq;
 #pragma unroll
                 for (int b = 0; b < D / 64; ++b)
                     tma_load_4d(ring + st * 2 * TB + b * (kAtKeys * 128), mk, b * 64, t0, at.kvh, sq, full + 8 * st);
@@ -634,13 +621,13 @@ __device__ __forceinline__ AttnRun attn_run(const AttnArgs &P, int j, int seq, i
     int unit, row, t = rt;
     if (!tc) {
         const int mt = own ? P.mt_own : P.mt_pre;
-        there = own ? own_tiles(P, seq) > 0 : P.mt_pre && P.prefix_len > P.cut_pre;
+        there = own ? own_tiles(P, seq) > 0 : P.mt_pre > 0;
         unit = (own ? nkv * P.mt_pre + seq * nkv * P.mt_own : 0) + kvh * mt + q / t;
         row = q % t;
     } else {
         const int two = own ? P.tc2_own : P.tc2_pre;
         t = two ? 128 : P.tc_rows;
-        there = (own ? P.tc_own && own_cut(P, seq) > 0 : P.tc_pre) && (two || !(j & 1));
+        there = (own ? P.tc_own && own_keys(P, seq) > 0 : P.tc_pre) && (two || !(j & 1));
         unit = (own ? nkv * P.tcm_pre + seq * nkv * P.tcm_own + kvh * P.tcm_own : kvh * P.tcm_pre) + q / t;
         row = q % t + (j & 1) * 128;
         t = P.tc_rows;

@@ -11,8 +11,9 @@
 // O / l.  With at most 128 row vectors both tiles hold the same ones and the key tiles go to them in turn.  D = 256 has
 // no room for a second O: there one tile alternates between two S.
 //
-// Only key tiles that every row sees come here (kernels_attn.cuh has the rest), so there are no masks, and every copy is in
-// bounds.  Work is dealt out like there: one line of key tiles, equal parts.
+// Only the last tiles of a problem have keys that some row does not see; there, S is masked after it was read, and what the
+// values of such keys may hold is taken out of the tile in shared memory before the product (0 x inf is not 0).  Work is
+// dealt out as in kernels_attn.cuh: one line of key tiles, equal parts.
 #pragma once
 #include "kernels_attn.cuh"
 
@@ -47,7 +48,7 @@ struct TcAt {
     int seq, kvh, mt, tile, tiles;
 };
 __device__ __forceinline__ int tc_tiles(const AttnArgs &P, int b) {
-    const int n = own_cut(P, b) / kTcKeys;
+    const int n = P.tc_own ? (own_keys(P, b) + kTcKeys - 1) / kTcKeys : 0;
     return n ? n + kTcEmpty : 0;
 }
 // The key tiles [t0, t0 + n) of the place's (problem, row tile) that lie in the next `left` tiles of the line; takes them off.
@@ -77,6 +78,7 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {  /
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 __device__ __forceinline__ void tile_sync(int w) { asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory"); }  // the warps of a row tile
+__device__ __forceinline__ uint32_t low32(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }  // n low bits
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -147,6 +149,8 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     __shared__ uint32_t s_tmem;
     __shared__ float s_top[2][T::TILES][2][128];  // a row's two maxima, by turns
     __shared__ int s_fail;
+    // New slots in which infinite or NaN values were met, a bit each.  Only a hint of where to look again: bits stay.
+    __shared__ unsigned s_odd[2];
     const int tid = threadIdx.x, warp = tid >> 5, c = blockIdx.x;
     uint8_t *base = tc_smem_raw + ((1024 - (smem_u32(tc_smem_raw) & 1023)) & 1023);
     const uint32_t q_s = smem_u32(base), ring_s = q_s + T::TILES * T::Q_BYTES;
@@ -157,6 +161,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     constexpr int kProducer = T::TILES * 8, kIssuer = kProducer + 1;
     if (tid == 0) {
         s_fail = 0;
+        s_odd[0] = s_odd[1] = 0;
         for (int i = 0; i < 2 * T::SLOTS; ++i) mbar_init(full + 8 * i, 1);
         for (int i = 0; i < T::TILES; ++i) {
             mbar_init(qfull + 8 * i, 8);
@@ -179,7 +184,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     const uint32_t tmem = s_tmem;
     griddep_wait();
     griddep_launch_dependents();  // (now, when all before this launch is done: the next one does not wait for it)
-    const int nkv = P.own.n_kv, per_seq = nkv * P.tcm_own, tp = P.tc_pre ? P.cut_pre / N + kTcEmpty : 0;
+    const int nkv = P.own.n_kv, per_seq = nkv * P.tcm_own, tp = P.tc_pre ? (P.prefix_len + N - 1) / N + kTcEmpty : 0;
     const long long line_pre = (long long)nkv * P.tcm_pre * tp;
     long long first = 0, end = 0;
     int seq = 0, off = 0;
@@ -302,6 +307,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
         const uint32_t flip = P.scale2 < 0.0f ? 0x80008000u : 0u;  // the sign of the scale goes into Q: scores only need a positive one
         const float scale = fabsf(P.scale2);
         int turn = 0;
+        RingAt<T::SLOTS> ring;  // the ring place of the segment's first K
         uint32_t sph[T::BUFS] = {}, oph = 0, pvph = 1;  // pvph: parity of the product before this tile's
         for (; left > 0; tc_next(P, at)) {
             int t0;
@@ -311,6 +317,10 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             const int mine = two ? (n + 1 - w) >> 1 : n;
             const int M = (at.seq < 0 ? P.S : P.rows) * P.G, row0 = at.seq < 0 ? 0 : at.seq * P.rows;
             const int r = two ? at.mt * 128 + row : at.mt * T::ROWS + w * 128 + row;
+            // keys below `seen` are seen by every row, new slots from `fresh` on by the row's bits, none from `keys` on
+            const int fresh = at.seq < 0 ? P.prefix_len : P.base[at.seq], keys = at.seq < 0 ? P.prefix_len : own_keys(P, at.seq);
+            const int seen = min(fresh, keys);
+            const unsigned long long bits = at.seq >= 0 && r < M ? row_mask(P, at.seq * P.rows + r / P.G, r / P.G) : 0;
             float m = -INFINITY, l = 0.0f;
             if (mine) {
                 // D / 8 lanes read a row together; a warp brings 16 of its 32 rows
@@ -349,16 +359,27 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                 float s[32];
                 tmem_ld32(region + T::S_COL + hf * 32, s);
                 tmem_wait_ld32(s);
+                const int j = two ? 2 * i + w : i, k0 = (t0 + j) * N, c0 = k0 + hf * 32;  // the tile's first key, this thread's
+                const bool open = k0 + N <= seen;
+                uint32_t see = 0xffffffffu;
+                if (!open) {
+                    const int d = c0 - fresh;
+                    const unsigned long long late = d >= 64 || d <= -32 ? 0ull : d >= 0 ? bits >> d : bits << -d;
+                    see = (low32(seen - c0) | (uint32_t)late) & low32(keys - c0);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) s[e] = (see >> e) & 1u ? s[e] : -INFINITY;
+                }
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
                 for (int e = 4; e < 32; ++e) mx[e & 3] = max_nan(mx[e & 3], s[e]);
-                float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * scale;
+                float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
+                top = see ? top * scale : -INFINITY;
                 // both halves of S have been read when both maxima are there: the weights may replace any of it
                 s_top[turn][w][hf][row] = top;
                 tile_sync(w);
                 top = max_nan(top, s_top[turn][w][hf ^ 1][row]);
                 turn ^= 1;
-                const bool plain = __all_sync(0xffffffffu, top < INFINITY);  // no NaN, no infinity
+                const bool plain = __all_sync(0xffffffffu, open && top < INFINITY);  // no mask, no NaN, no infinity
                 if (i == 0) {
                     m = top;
                 } else if (__any_sync(0xffffffffu, top > m + kAtLag)) {
@@ -387,10 +408,35 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                 }
                 pvph ^= 1u;
                 if (P.scores && at.seq >= 0 && r < M) {
-                    float *x = P.scores + (((long long)at.seq * nkv + at.kvh) * M + r) * P.own.cap +
-                               (long long)(t0 + (two ? 2 * i + w : i)) * N + hf * 32;
+                    float *x = P.scores + (((long long)at.seq * nkv + at.kvh) * M + r) * P.own.cap + c0;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] = s[e] * scale;
+                    for (int e = 0; e < 32; ++e)
+                        if (c0 + e < keys) x[e] = (see >> e) & 1u ? s[e] * scale : -INFINITY;
+                }
+                if (!open && at.seq >= 0) {
+                    // values of slots that are not seen by all: zeros for those never stored, and for what is not finite (rows
+                    // that do see such a value add it when the partial result is written)
+                    RingAt<T::SLOTS> at_v = ring;
+                    at_v.skip(2 * j + 1);
+                    um_spin(full + 8 * at_v.i, at_v.ph, fail);
+                    uint8_t *vt = base + (ring_s - q_s) + at_v.i * T::TILE_BYTES;
+                    for (int x = tid & 255; x < N * (D / 8); x += 256) {
+                        const int key = x / (D / 8), ch = x % (D / 8);
+                        if (k0 + key < seen) continue;
+                        uint4 *at_x = reinterpret_cast<uint4 *>(vt + (ch >> 3) * (N * 128) + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (k0 + key < keys) {
+                            const uint4 o = *at_x;
+                            v = make_uint4(finite16<BF16>(o.x), finite16<BF16>(o.y), finite16<BF16>(o.z), finite16<BF16>(o.w));
+                            const int b = k0 + key - fresh;
+                            if ((o.x ^ v.x) | (o.y ^ v.y) | (o.z ^ v.z) | (o.w ^ v.w)) {
+                                atomicOr(&s_odd[b >> 5], 1u << (b & 31));
+                                __threadfence_block();  // the other row tile, which finds the zeros, finds the bit
+                            }
+                        }
+                        *at_x = v;
+                    }
+                    fence_proxy_async();
                 }
                 const float ms = (m == -INFINITY ? 0.0f : m) - kAtLift<BF16>;
                 const uint64_t scales = pack2(scale, scale), shift = pack2(-ms, -ms);
@@ -414,7 +460,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                         }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] = ex2(fmaf(x[e], scale, -ms));
+                        for (int e = 0; e < 32; ++e) x[e] = (see >> e) & 1u ? ex2(fmaf(x[e], scale, -ms)) : 0.0f;
 #pragma unroll
                         for (int e = 0; e < 16; ++e) sums[e & 1] = add2(sums[e & 1], pack2(x[2 * e], x[2 * e + 1]));
                     }
@@ -458,6 +504,9 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             tile_sync(w);
             if (hf == 0 && r < M) P.ml[to + row] = make_float2(m, l + s_top[turn][w][1][row]);
             turn ^= 1;
+            const int late = keys - fresh;  // new slots there are
+            const unsigned long long there = late >= 64 ? ~0ull : late <= 0 ? 0ull : (1ull << late) - 1;
+            const unsigned long long odd = (s_odd[0] | (unsigned long long)s_odd[1] << 32) & bits & there;
             // A thread has a row's dims, a store wants a row's dims in neighbouring lanes: 32 rows x 16 dims at a time turn in
             // the shared memory of this row tile's query vectors, whose products are done.
             uint8_t *swap = base + w * T::Q_BYTES + (warp & 7) * 2048;
@@ -470,6 +519,15 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                 } else {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+                }
+                for (unsigned long long q = odd; q; q &= q - 1) {
+                    const uint16_t *v = P.own.v + (long long)at.seq * P.own.seq_stride + at.kvh * P.own.head_stride +
+                                        ((long long)fresh + __ffsll(q) - 1) * P.own.slot_stride + d;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float x = from16<BF16>(v[e]);
+                        if (!isfinite(x)) o[e] += x;
+                    }
                 }
                 __syncwarp();
 #pragma unroll
@@ -484,6 +542,8 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                 }
             }
             tile_sync(w);  // before new query vectors replace what another warp still turns
+            ring.skip(2 * n % T::SLOTS);
+            if ((2 * n / T::SLOTS) & 1) ring.ph ^= 1u;
             tmem_fence_before();
         }
     }

@@ -241,6 +241,36 @@ def test_values_that_no_row_may_see(dev, T, D):
         assert np.all(np.isposinf(out[s, :, 3]) == want_inf) and np.all(np.isfinite(np.delete(out[s], 3, 1)))
 
 
+@pytest.mark.parametrize("T, D, heads", [("bf16", 64, 8), ("f16", 128, 24), ("bf16", 256, 12), ("f16", 64, 48)])
+def test_values_that_no_row_may_see_with_many_rows(dev, T, D, heads):
+    """The same where a sequence's rows fill tiles of 128 (one, two and more of them), with slots past every length spoilt."""
+    n, r, cap, base, hidden = 3, 9, 210, [60, 3, 201], 5
+    mask = [(1 << r) - 1 & ~(1 << hidden)] * (n * r)
+
+    def spoil(q, k, v, pk, pv):
+        for b in range(n):
+            t = base[b] + hidden
+            k[b, :, t, ::2], k[b, :, t, 1::2] = float("nan"), float("inf")
+            v[b, :, t, ::2], v[b, :, t, 1::2] = float("-inf"), float("nan")
+
+    clean, a0 = run_attention(3, n, r, heads, 2, D, T, cap, base, Tp=90, mask=mask, acc=True)
+    out, a1 = run_attention(3, n, r, heads, 2, D, T, cap, base, Tp=90, mask=mask, acc=True, prepare=spoil, check=False)
+    assert np.array_equal(out, clean) and np.array_equal(a0, a1)
+    seen = [m | (1 << hidden) if i % r >= 6 else m for i, m in enumerate(mask)]
+
+    def spoil_v(q, k, v, pk, pv):
+        for b in range(n):
+            v[b, :, base[b] + hidden, 3] = float("inf")
+
+    out, _ = run_attention(3, n, r, heads, 2, D, T, cap, base, Tp=90, mask=seen, prepare=spoil_v, check=False)
+    for s in range(n * r):
+        want_inf = s % r >= 6
+        assert np.all(np.isposinf(out[s, :, 3]) == want_inf) and np.all(np.isfinite(np.delete(out[s], 3, 1)))
+    none = [0] * (n * r)
+    out, _ = run_attention(4, n, r, heads, 2, D, T, r + 3, [0, 0, 0], mask=none, acc=True)
+    assert np.all(out == 0.0)
+
+
 def test_attention_large_scores(dev):
     """Scores of hundreds: the softmax is a single slot, and nothing overflows."""
     run_attention(1, 2, 1, 4, 2, 64, "f16", 300, [299, 50], Tp=100, q_std=40.0, scale=1.0, acc=True)
