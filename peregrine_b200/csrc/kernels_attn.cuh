@@ -22,6 +22,7 @@ constexpr int kAtKeys = 64;      // keys of a tile
 constexpr int kAtThreads = 160;  // 4 warps with 16 keys of a tile each, one that issues the copies
 constexpr int kAtCombine = 128;
 constexpr int kTcKeys = 64;  // keys of a tile of the tensor-memory kernel
+constexpr int kAtMany = 16;     // row vectors of a problem up to which the joining launch adds up the weights itself
 constexpr int kAtChunk = 1024;  // slots whose weights one CTA adds up
 
 struct AttnArgs {
@@ -50,6 +51,7 @@ struct AttnArgs {
     long long tc_row0;      // first row of the tensor-memory kernel's
     int2 *cta_of, *tc_cta_of;  // per unit: the CTAs that have its first and its last tile
     float *scores;  // [n_seq][n_kv][rows * G][cap]: x of the own slots (-inf: not seen); only with acc
+    float2 *stats;  // [S * H]: m and 1 / l of every row vector, joined; only with acc and many rows
 };
 
 template <bool BF16>
@@ -688,7 +690,9 @@ __device__ __forceinline__ void attn_row(const AttnArgs &P, AttnRow &R, int lane
 }
 
 // Joins the partials.  The first `row_ctas` CTAs take 4 / WPR row vectors each, WPR warps to one (4 where there are too few
-// row vectors to fill the device); with acc, further CTAs take 1024 slots of one (sequence, kv head) each.
+// row vectors to fill the device); with acc and up to kAtMany row vectors a problem, further CTAs take 1024 slots of one
+// (sequence, kv head) each.  What bounds it is the partials' way from the second-level cache (22 of 512 bytes a row vector in
+// a batch of 32 behind a prefix of 32768: 23 MB in 7 us; eight loads under way instead of one took no less).
 template <int D, bool BF16, int WPR>
 __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P, int rt, int row_ctas, int chunks) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -740,6 +744,7 @@ __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P,
             }
         }
         const float inv = R.l == 0.0f ? 0.0f : 1.0f / R.l;
+        if (P.stats && lane == 0) P.stats[u] = make_float2(R.m - kAtLift<BF16>, inv);
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] *= inv;
         const long long to = (long long)u * D + lane * E;
@@ -760,32 +765,62 @@ __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P,
     const int t0 = chunk * kAtChunk + threadIdx.x;
     if (chunk * kAtChunk >= keys) return;
     constexpr int C = kAtChunk / kAtCombine;
-    __shared__ float2 s_row[64];  // m and 1 / l of the row vectors
+    __shared__ float2 s_row[kAtMany];  // m and 1 / l of the row vectors
     const int M = P.rows * P.G;
     float sum[C] = {};
-    for (int r0 = 0; r0 < M; r0 += 64) {
-        if (r0) __syncthreads();
-        for (int r = r0 + warp; r < min(M, r0 + 64); r += 4) {
-            AttnRow R;
-            attn_row(P, R, lane, seq, kvh, r, rt);
-            if (lane == 0) s_row[r - r0] = make_float2(R.m - kAtLift<BF16>, R.l == 0.0f ? 0.0f : 1.0f / R.l);
-        }
-        __syncthreads();
-        const float *x = P.scores + ((long long)g * M + r0) * P.own.cap + t0;
-        for (int r = 0; r < min(M - r0, 64); ++r, x += P.own.cap) {
-            const float2 st = s_row[r];
-            float w[C];
+    for (int r = warp; r < M; r += 4) {
+        AttnRow R;
+        attn_row(P, R, lane, seq, kvh, r, rt);
+        if (lane == 0) s_row[r] = make_float2(R.m - kAtLift<BF16>, R.l == 0.0f ? 0.0f : 1.0f / R.l);
+    }
+    __syncthreads();
+    const float *x = P.scores + (long long)g * M * P.own.cap + t0;
+    for (int r = 0; r < M; ++r, x += P.own.cap) {
+        const float2 st = s_row[r];
+        float w[C];
 #pragma unroll
-            for (int j = 0; j < C; ++j) w[j] = t0 + j * kAtCombine < keys ? x[j * kAtCombine] : -INFINITY;
+        for (int j = 0; j < C; ++j) w[j] = t0 + j * kAtCombine < keys ? x[j * kAtCombine] : -INFINITY;
 #pragma unroll
-            for (int j = 0; j < C; ++j)
-                if (w[j] != -INFINITY) sum[j] = fmaf(ex2(w[j] - st.x), st.y, sum[j]);
-        }
+        for (int j = 0; j < C; ++j)
+            if (w[j] != -INFINITY) sum[j] = fmaf(ex2(w[j] - st.x), st.y, sum[j]);
     }
     float *acc = P.own.acc + (long long)g * P.own.cap + t0;
 #pragma unroll
     for (int j = 0; j < C; ++j)
         if (t0 + j * kAtCombine < keys) acc[j * kAtCombine] += sum[j];
+}
+
+// The same for problems of many row vectors: 64 slots of one (sequence, kv head) a CTA, the row vectors dealt to its eight
+// warps, whose sums are added in order.
+__global__ void __launch_bounds__(256) attn_acc_kernel(const AttnArgs P, int chunks) {
+    griddep_wait();
+    griddep_launch_dependents();
+    const int g = blockIdx.x / chunks, chunk = blockIdx.x % chunks, seq = g / P.own.n_kv, kvh = g % P.own.n_kv;
+    const int keys = own_keys(P, seq), M = P.rows * P.G, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int t0 = chunk * 64 + lane;
+    if (chunk * 64 >= keys) return;
+    const float *x = P.scores + (long long)g * M * P.own.cap + t0;
+    const float2 *stats = P.stats + (long long)seq * P.rows * P.H + kvh * P.G;
+    float sum[2] = {};
+#pragma unroll 4
+    for (int r = warp; r < M; r += 8) {
+        const float2 st = stats[(long long)(r / P.G) * P.H + r % P.G];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float w = t0 + j * 32 < keys ? x[(long long)r * P.own.cap + j * 32] : -INFINITY;
+            if (w != -INFINITY) sum[j] = fmaf(ex2(w - st.x), st.y, sum[j]);
+        }
+    }
+    __shared__ float s_sum[8][2][32];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s_sum[warp][j][lane] = sum[j];
+    __syncthreads();
+    if (warp >= 2) return;
+    float all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) all += s_sum[w][warp][lane];
+    const int t = chunk * 64 + warp * 32 + lane;
+    if (t < keys) P.own.acc[(long long)g * P.own.cap + t] += all;
 }
 
 }  // namespace pgb

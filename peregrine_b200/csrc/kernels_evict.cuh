@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
 // part of the slots in shared memory, histograms and counts are read across the cluster.  One CTA alone reads at about
 // 100 GB/s and sweeps 40000 slots six times in 108 us; eight take 8.
 constexpr int kEvCluster = 8, kEvPartThreads = 512, kEvPartMost = 32768;  // slots of a CTA at the most
-constexpr int kEvAlone = 4096;                                            // up to here one CTA is a cluster
+constexpr int kEvAlone = 1024;                                            // up to here one CTA is a cluster
 
 template <int C>
 __device__ __forceinline__ void cluster_sync() {
