@@ -153,7 +153,7 @@ struct NormRopeLaunch {
 };
 
 // Problems with more row vectors than this go to the tensor-memory kernel, whose tiles have 128 rows.
-constexpr int kTcRows = 16;
+constexpr int kTcRows = kAtMany;
 
 // Row tile of the split kernel.
 int row_tile(int rows, int H, int n_kv) { return rows * (H / n_kv) <= 8 ? 8 : 16; }
@@ -199,7 +199,7 @@ size_t attn_plan(AttnArgs *P, const KvArgs &own, int S, int H, int prefix_len, i
     P->ml = reinterpret_cast<float2 *>(take((split_rows + tc_rows) * 8));
     P->cta_of = reinterpret_cast<int2 *>(take((size_t)units * 8));
     P->tc_cta_of = reinterpret_cast<int2 *>(take((size_t)tc_units * 8));
-    P->scores = own.acc ? reinterpret_cast<float *>(take((size_t)own.n_seq * own.n_kv * m_own * own.cap * 4)) : nullptr;
+    P->scores = own.acc ? reinterpret_cast<float *>(take((size_t)own.n_seq * own.n_kv * m_own * (((size_t)own.cap + 3) / 4) * 16)) : nullptr;
     P->stats = own.acc ? reinterpret_cast<float2 *>(take((size_t)S * H * 8)) : nullptr;
     return at;
 }
@@ -255,13 +255,13 @@ struct AttnLaunch {
         }
         // waits on the device for the end of the launches before
         const int vectors = P.S * P.H, groups = P.own.n_seq * P.own.n_kv;
-        const bool few = vectors < 4 * P.tc_ctas, many = P.rows * P.G > kAtMany;
+        const bool few = vectors < 4 * P.tc_ctas, many = P.tc_own;
         const int row_ctas = few ? vectors : (vectors + 3) / 4, chunks = P.own.acc && !many ? (P.own.cap + kAtChunk - 1) / kAtChunk : 0;
         if (!launch_early(few ? attn_join_kernel<D, BF16, 4> : attn_join_kernel<D, BF16, 1>, (unsigned)(row_ctas + chunks * groups), kAtCombine,
                           0, stream, "attention join launch", 1, true, P, RT, row_ctas, chunks))
             return 0;
         if (!P.own.acc || !many) return 1;
-        const int parts = (P.own.cap + 63) / 64;
+        const int parts = (P.own.cap + 31) / 32;
         return launch_early(attn_acc_kernel, (unsigned)(parts * groups), 256, 0, stream, "attention weights launch", 1, true, P, parts);
     }
     template <int D, bool BF16>
@@ -337,7 +337,7 @@ PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, 
     if (!kv_args(&P.own, own, what) || !rows_ok(S, H, P.own, rows_per_seq, what)) return 0;
     if (rows_per_seq > 64) return refuse("%s: %d rows of a sequence are more than 64", what, rows_per_seq);
     if (H % own->n_kv) return refuse("%s: %d heads are no multiple of %d", what, H, own->n_kv);
-    if ((long long)S * H > 0x3fffffff || (own->acc && ((long long)own->cap / 64 + 1) * own->n_seq * own->n_kv > 0x3fffffff))
+    if ((long long)S * H > 0x3fffffff || (own->acc && ((long long)own->cap / 32 + 1) * own->n_seq * own->n_kv > 0x3fffffff))
         return refuse("%s: too many rows and heads", what);
     if (!out_dev || !q_dev || !base_dev || !work_dev) return refuse("%s: null pointer", what);
     if (!aligned(out_dev, 16) || !aligned(q_dev, 16) || !aligned(base_dev, 4) || !aligned(mask_dev, 8) || !aligned(work_dev, 256))

@@ -50,7 +50,9 @@ struct AttnArgs {
     float2 *ml;     // one per row of part: m and l
     long long tc_row0;      // first row of the tensor-memory kernel's
     int2 *cta_of, *tc_cta_of;  // per unit: the CTAs that have its first and its last tile
-    float *scores;  // [n_seq][n_kv][rows * G][cap]: x of the own slots (-inf: not seen); only with acc
+    // x of the own slots (-inf: not seen), only with acc: [n_seq][n_kv][rows * G][cap] from the split kernel,
+    // [n_seq][n_kv][cap / 4, rounded up][rows * G][4] from the tensor-memory kernel, whose lanes hold neighbouring rows
+    float *scores;
     float2 *stats;  // [S * H]: m and 1 / l of every row vector, joined; only with acc and many rows
 };
 
@@ -68,6 +70,10 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ int own_keys(const AttnArgs &P, int b) {
     const int base = P.base[b];
     return base < 0 ? 0 : (int)min((long long)base + P.rows, (long long)P.own.cap);
+}
+// Where the tensor-memory kernel's scores of slot 4 q and the three behind it with row vector r stand.
+__device__ __forceinline__ float *score_at(const AttnArgs &P, int g, int q, int M, int r) {
+    return P.scores + (((long long)g * ((P.own.cap + 3) >> 2) + q) * M + r) * 4;
 }
 // New slots that row i of a sequence sees, a bit each.
 __device__ __forceinline__ unsigned long long row_mask(const AttnArgs &P, int row, int i) {
@@ -149,15 +155,16 @@ __device__ __forceinline__ int attn_unit(const AttnArgs &P, const AttnAt &a) {
     return a.seq < 0 ? a.kvh * P.mt_pre + a.mt
                      : P.own.n_kv * P.mt_pre + (a.seq * P.own.n_kv + a.kvh) * P.mt_own + a.mt;
 }
-// Where CTA c's part begins.  No more CTAs share the line than it has tiles, so that no part is empty.
+// Where CTA c's part begins.  No more CTAs share the line than leave each `least` tiles: none is empty, and the shorter the
+// parts, the more partial results there are to join.
 __device__ __forceinline__ long long line_part(long long total, int ctas, int c) { return total * c / ctas; }
-__device__ __forceinline__ int line_ctas(long long total, int ctas) { return (int)min((long long)ctas, max(total, 1ll)); }
+__device__ __forceinline__ int line_ctas(long long total, int ctas, int least) { return (int)min((long long)ctas, max(total / least, 1ll)); }
 
 // This CTA's part [first, end) of a line made of `line_pre` tiles of the prefix and, per sequence, tiles_of(b) * per_seq
 // own ones; `seq` and `off` (tiles of the sequences before it): the sequence of the first tile, where it is an own one.
 // False: no tile is this CTA's.  W: warps of the CTA, all of which call.
 template <int W, typename F>
-__device__ __forceinline__ bool line_share(int ns, F tiles_of, int per_seq, long long line_pre, int ctas, long long &first,
+__device__ __forceinline__ bool line_share(int ns, F tiles_of, int per_seq, long long line_pre, int ctas, int least, long long &first,
                                            long long &end, int &seq, int &off) {
     __shared__ int s_sum[W], s_seq, s_off;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = blockIdx.x;
@@ -174,7 +181,7 @@ __device__ __forceinline__ bool line_share(int ns, F tiles_of, int per_seq, long
         for (int w = 0; w < W; ++w) units += s_sum[w];
     }
     const long long total = line_pre + units * per_seq;
-    const int nc = line_ctas(total, ctas);
+    const int nc = line_ctas(total, ctas, least);
     if (c >= nc) return false;
     first = line_part(total, nc, c);
     end = line_part(total, nc, c + 1);
@@ -451,7 +458,7 @@ __global__ void __launch_bounds__(kAtThreads, SplitShape<D, RT>::PER_SM)
     const long long line_pre = (long long)nkv * P.mt_pre * tp;
     long long first, end;
     int seq = 0, off = 0;
-    if (!line_share<kAtThreads / 32>(P.own.n_seq, [&](int b) { return own_tiles(P, b); }, per_seq, line_pre, P.ctas, first, end, seq, off)) {
+    if (!line_share<kAtThreads / 32>(P.own.n_seq, [&](int b) { return own_tiles(P, b); }, per_seq, line_pre, P.ctas, 1, first, end, seq, off)) {
         griddep_wait();
         return;
     }
@@ -689,6 +696,14 @@ __device__ __forceinline__ void attn_row(const AttnArgs &P, AttnRow &R, int lane
     R.l = l;
 }
 
+// Adds the weights 2^(x - m) / l of four slots to their sums.
+__device__ __forceinline__ void attn_weigh(float (&sum)[4], const float4 &x, const float2 &st) {
+    if (x.x != -INFINITY) sum[0] = fmaf(ex2(x.x - st.x), st.y, sum[0]);
+    if (x.y != -INFINITY) sum[1] = fmaf(ex2(x.y - st.x), st.y, sum[1]);
+    if (x.z != -INFINITY) sum[2] = fmaf(ex2(x.z - st.x), st.y, sum[2]);
+    if (x.w != -INFINITY) sum[3] = fmaf(ex2(x.w - st.x), st.y, sum[3]);
+}
+
 // Joins the partials.  The first `row_ctas` CTAs take 4 / WPR row vectors each, WPR warps to one (4 where there are too few
 // row vectors to fill the device); with acc and up to kAtMany row vectors a problem, further CTAs take 1024 slots of one
 // (sequence, kv head) each.  What bounds it is the partials' way from the second-level cache (22 of 512 bytes a row vector in
@@ -762,18 +777,17 @@ __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P,
     const int u = blockIdx.x - row_ctas, g = u / chunks, chunk = u % chunks;
     const int seq = g / P.own.n_kv, kvh = g % P.own.n_kv;
     const int keys = own_keys(P, seq);
-    const int t0 = chunk * kAtChunk + threadIdx.x;
     if (chunk * kAtChunk >= keys) return;
     constexpr int C = kAtChunk / kAtCombine;
     __shared__ float2 s_row[kAtMany];  // m and 1 / l of the row vectors
-    const int M = P.rows * P.G;
-    float sum[C] = {};
+    const int M = P.rows * P.G, t0 = chunk * kAtChunk + threadIdx.x;
     for (int r = warp; r < M; r += 4) {
         AttnRow R;
         attn_row(P, R, lane, seq, kvh, r, rt);
         if (lane == 0) s_row[r] = make_float2(R.m - kAtLift<BF16>, R.l == 0.0f ? 0.0f : 1.0f / R.l);
     }
     __syncthreads();
+    float sum[C] = {};
     const float *x = P.scores + (long long)g * M * P.own.cap + t0;
     for (int r = 0; r < M; ++r, x += P.own.cap) {
         const float2 st = s_row[r];
@@ -790,37 +804,24 @@ __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P,
         if (t0 + j * kAtCombine < keys) acc[j * kAtCombine] += sum[j];
 }
 
-// The same for problems of many row vectors: 64 slots of one (sequence, kv head) a CTA, the row vectors dealt to its eight
-// warps, whose sums are added in order.
+// The same for problems of many row vectors: a warp takes four slots of one (sequence, kv head), its lanes the row vectors.
 __global__ void __launch_bounds__(256) attn_acc_kernel(const AttnArgs P, int chunks) {
     griddep_wait();
     griddep_launch_dependents();
-    const int g = blockIdx.x / chunks, chunk = blockIdx.x % chunks, seq = g / P.own.n_kv, kvh = g % P.own.n_kv;
-    const int keys = own_keys(P, seq), M = P.rows * P.G, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int t0 = chunk * 64 + lane;
-    if (chunk * 64 >= keys) return;
-    const float *x = P.scores + (long long)g * M * P.own.cap + t0;
+    const int g = blockIdx.x / chunks, q = blockIdx.x % chunks * 8 + (threadIdx.x >> 5), seq = g / P.own.n_kv, kvh = g % P.own.n_kv;
+    const int keys = own_keys(P, seq), M = P.rows * P.G, lane = threadIdx.x & 31;
+    if (4 * q >= keys) return;
     const float2 *stats = P.stats + (long long)seq * P.rows * P.H + kvh * P.G;
-    float sum[2] = {};
+    float sum[4] = {};
 #pragma unroll 4
-    for (int r = warp; r < M; r += 8) {
-        const float2 st = stats[(long long)(r / P.G) * P.H + r % P.G];
+    for (int r = lane; r < M; r += 32)
+        attn_weigh(sum, *reinterpret_cast<const float4 *>(score_at(P, g, q, M, r)), stats[(long long)(r / P.G) * P.H + r % P.G]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float w = t0 + j * 32 < keys ? x[(long long)r * P.own.cap + j * 32] : -INFINITY;
-            if (w != -INFINITY) sum[j] = fmaf(ex2(w - st.x), st.y, sum[j]);
-        }
-    }
-    __shared__ float s_sum[8][2][32];
+    for (int e = 0; e < 4; ++e)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) s_sum[warp][j][lane] = sum[j];
-    __syncthreads();
-    if (warp >= 2) return;
-    float all = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) all += s_sum[w][warp][lane];
-    const int t = chunk * 64 + warp * 32 + lane;
-    if (t < keys) P.own.acc[(long long)g * P.own.cap + t] += all;
+        for (int o = 16; o > 0; o >>= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
+    const int t = 4 * q + lane;
+    if (lane < 4 && t < keys) P.own.acc[(long long)g * P.own.cap + t] += lane == 0 ? sum[0] : lane == 1 ? sum[1] : lane == 2 ? sum[2] : sum[3];
 }
 
 }  // namespace pgb

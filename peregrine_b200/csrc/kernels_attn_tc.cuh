@@ -22,6 +22,7 @@ namespace pgb {
 // Tiles that a change of the problem costs a CTA (query vectors, first and last tile, its partial result): on the line every
 // (problem, row tile) begins with so many empty ones.
 constexpr int kTcEmpty = 8;
+constexpr int kTcLeast = 4;  // tiles (empty ones too) of a CTA at least
 
 template <int D, bool BF16, bool F32>
 struct TcShape {
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     const long long line_pre = (long long)nkv * P.tcm_pre * tp;
     long long first = 0, end = 0;
     int seq = 0, off = 0;
-    if (!line_share<T::THREADS / 32>(P.own.n_seq, [&](int b) { return tc_tiles(P, b); }, per_seq, line_pre, P.tc_ctas, first, end, seq,
+    if (!line_share<T::THREADS / 32>(P.own.n_seq, [&](int b) { return tc_tiles(P, b); }, per_seq, line_pre, P.tc_ctas, kTcLeast, first, end, seq,
                                      off))
         first = end = 0;
     TcAt at;
@@ -408,10 +409,14 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                 }
                 pvph ^= 1u;
                 if (P.scores && at.seq >= 0 && r < M) {
-                    float *x = P.scores + (((long long)at.seq * nkv + at.kvh) * M + r) * P.own.cap + c0;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (c0 + e < keys) x[e] = (see >> e) & 1u ? s[e] * scale : -INFINITY;
+                    for (int e = 0; e < 32; e += 4) {
+                        float x[4];
+#pragma unroll
+                        for (int f = 0; f < 4; ++f) x[f] = (see >> (e + f)) & 1u ? s[e + f] * scale : -INFINITY;
+                        if (c0 + e < keys)
+                            *reinterpret_cast<float4 *>(score_at(P, at.seq * nkv + at.kvh, (c0 + e) >> 2, M, r)) = make_float4(x[0], x[1], x[2], x[3]);
+                    }
                 }
                 if (!open && at.seq >= 0) {
                     // values of slots that are not seen by all: zeros for those never stored, and for what is not finite (rows
