@@ -130,6 +130,13 @@ template <int n>
 struct RingAt {
     int i = 0;
     uint32_t ph = 0;
+    __device__ __forceinline__ void next(int k) {  // k < n
+        i += k;
+        if (i >= n) {
+            i -= n;
+            ph ^= 1u;
+        }
+    }
     __device__ __forceinline__ void skip(int k) {
         i += k;
         while (i >= n) {
@@ -223,7 +230,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
 #pragma unroll
                         for (int b = 0; b < DB; ++b)
                             tma_load_4d(ring_s + r.i * T::TILE_BYTES + b * (N * 128), v ? mv : mk, b * 64, (t0 + j) * N, at.kvh, s, full + 8 * r.i);
-                        r.skip(1);
+                        r.next(1);
                         if (!begun && v) {
                             // The query vectors' loads must not queue behind a ring full of tiles.  (With three tiles to come
                             // the barrier stays in this phase until they do.)
@@ -241,61 +248,72 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             constexpr uint32_t kIdescS = (1u << 4) | kType | ((uint32_t)(N >> 3) << 17) | (8u << 24);
             constexpr uint32_t kIdescO = (1u << 4) | kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);  // V: dims contiguous
             RingAt<T::SLOTS> seg;  // the ring place of the segment's first K
-            uint32_t qph = 0, pph[T::TILES][T::BUFS] = {};
+            uint32_t qph = 0, pph = 0;
             for (; left > 0 && !*fail; tc_next(P, at)) {
                 int t0;
                 const int n = tc_segment(at, left, t0);
                 const int two = T::TILES == 2 && (at.seq < 0 ? P.tc2_pre : P.tc2_own);
                 // tile i of row tile w is key tile `i` of the segment, or 2 i + w when they take turns
-                auto count = [&](int w) { return two ? (n + 1 - w) >> 1 : n; };
-                auto place = [&](int w, int i, int v) {
-                    RingAt<T::SLOTS> r = seg;
-                    r.skip(2 * (two ? 2 * i + w : i) + v);
-                    return r;
-                };
+                const int step = two ? 4 : 2;
+                int count[T::TILES], most = 0;
+                RingAt<T::SLOTS> kp[T::TILES], vp[T::TILES];  // of the row tiles' next K and V
+#pragma unroll
+                for (int w = 0; w < T::TILES; ++w) {
+                    count[w] = two ? (n + 1 - w) >> 1 : n;
+                    most = max(most, count[w]);
+                    kp[w] = seg;
+                    if (two && w) kp[w].next(2);
+                    vp[w] = kp[w];
+                    vp[w].next(1);
+                }
                 auto scores = [&](int w, int i) {
-                    const RingAt<T::SLOTS> r = place(w, i, 0);
+                    const RingAt<T::SLOTS> r = kp[w];
+                    kp[w].next(step);
                     if (i == 0) um_spin(qfull + 8 * w, (qph >> w) & 1u, fail);
                     if (w == 0 || two) um_spin(full + 8 * r.i, r.ph, fail);
                     tmem_fence_after();
                     const uint32_t d = tmem + (w * T::BUFS + i % T::BUFS) * T::BUF_COLS + T::S_COL;
+                    const uint64_t qd = desc_sw128(q_s + w * T::Q_BYTES, 16), kd = desc_sw128(ring_s + r.i * T::TILE_BYTES, 16);
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k)
-                        umma_f16_ss(d, desc_sw128(q_s + w * T::Q_BYTES + (k >> 2) * (128 * 128), 16) + (k & 3) * 2,
-                                    desc_sw128(ring_s + r.i * T::TILE_BYTES + (k >> 2) * (N * 128), 16) + (k & 3) * 2, kIdescS, k > 0);
+                        umma_f16_ss(d, qd + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2, kd + (k >> 2) * (N * 128 / 16) + (k & 3) * 2, kIdescS, k > 0);
                     if (w == T::TILES - 1 || two) umma_commit(empty + 8 * r.i);
                     umma_commit(sfull + 8 * (w * T::BUFS + i % T::BUFS));
                 };
-                int most = 0;
+#pragma unroll
                 for (int b = 0; b < T::BUFS; ++b)
+#pragma unroll
                     for (int w = 0; w < T::TILES; ++w)
-                        if (b < count(w)) scores(w, b);
-                for (int w = 0; w < T::TILES; ++w) {
-                    most = max(most, count(w));
-                    if (count(w)) qph ^= 1u << w;
-                }
+                        if (b < count[w]) scores(w, b);
+#pragma unroll
+                for (int w = 0; w < T::TILES; ++w)
+                    if (count[w]) qph ^= 1u << w;
                 for (int i = 0; i < most && !*fail; ++i)
 #pragma unroll
                     for (int w = 0; w < T::TILES; ++w) {
-                        if (i >= count(w)) continue;
-                        const RingAt<T::SLOTS> r = place(w, i, 1);
-                        const int buf = w * T::BUFS + i % T::BUFS;
-                        um_spin(pfull + 8 * buf, pph[w][i % T::BUFS], fail);
-                        pph[w][i % T::BUFS] ^= 1u;
+                        if (i >= count[w]) continue;
+                        const RingAt<T::SLOTS> r = vp[w];
+                        vp[w].next(step);
+                        const int bi = i % T::BUFS, buf = w * T::BUFS + bi;
+                        um_spin(pfull + 8 * buf, (pph >> buf) & 1u, fail);
+                        pph ^= 1u << buf;
                         if (w == 0 || two) um_spin(full + 8 * r.i, r.ph, fail);
                         tmem_fence_after();
+                        const uint64_t vd = desc_sw128(ring_s + r.i * T::TILE_BYTES, N * 128);
+                        const uint32_t pa = tmem + buf * T::BUF_COLS;
 #pragma unroll
                         for (int k = 0; k < N / 16; ++k)
 #pragma unroll
                             for (int t = 0; t < T::TERMS; ++t)
-                                umma_f16_ts(tmem + T::O_COL + w * D, tmem + buf * T::BUF_COLS + (k >> 1) * (16 * T::TERMS) + t * 16 + (k & 1) * 8,
-                                            desc_sw128(ring_s + r.i * T::TILE_BYTES + k * 2048, N * 128), kIdescO, i > 0 || k > 0 || t > 0);
+                                umma_f16_ts(tmem + T::O_COL + w * D, pa + (k >> 1) * (16 * T::TERMS) + t * 16 + (k & 1) * 8, vd + k * (2048 / 16),
+                                            kIdescO, i > 0 || k > 0 || t > 0);
                         if (w == T::TILES - 1 || two) umma_commit(empty + 8 * r.i);
-                        if (T::BUFS > 1) umma_commit(pvdone + 8 * w);
-                        if (i + 1 == count(w))
+                        if (i + 1 == count[w]) {
                             umma_commit(odone + 8 * w);
-                        else if (i + T::BUFS < count(w))
-                            scores(w, i + T::BUFS);
+                        } else {
+                            if (T::BUFS > 1) umma_commit(pvdone + 8 * w);
+                            if (i + T::BUFS < count[w]) scores(w, i + T::BUFS);
+                        }
                     }
                 seg.skip(2 * n % T::SLOTS);
                 if ((2 * n / T::SLOTS) & 1) seg.ph ^= 1u;
@@ -309,7 +327,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
         const float scale = fabsf(P.scale2);
         int turn = 0;
         RingAt<T::SLOTS> ring;  // the ring place of the segment's first K
-        uint32_t sph[T::BUFS] = {}, oph = 0, pvph = 1;  // pvph: parity of the product before this tile's
+        uint32_t sph[T::BUFS] = {}, oph = 0, pvph = 1;  // pvph: parity of the product before this tile's (the segment's last one is told by odone)
         for (; left > 0; tc_next(P, at)) {
             int t0;
             const int n = tc_segment(at, left, t0);
@@ -381,6 +399,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                 top = max_nan(top, s_top[turn][w][hf ^ 1][row]);
                 turn ^= 1;
                 const bool plain = __all_sync(0xffffffffu, open && top < INFINITY);  // no mask, no NaN, no infinity
+                if (i) pvph ^= 1u;
                 if (i == 0) {
                     m = top;
                 } else if (__any_sync(0xffffffffu, top > m + kAtLag)) {
@@ -407,7 +426,6 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                         }
                     }
                 }
-                pvph ^= 1u;
                 if (P.scores && at.seq >= 0 && r < M) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
