@@ -78,11 +78,17 @@ __device__ __forceinline__ void tc_next(const AttnArgs &P, TcAt &a) {
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {  // 128-byte swizzle, 8-row groups 1024 bytes apart
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void tile_sync(int w) { asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory"); }  // the warps of a row tile
+__device__ __forceinline__ void tile_sync(int w) { asm volatile("bar.sync %0, 256;" ::"r"(9 + w) : "memory"); }  // the warps of a row tile
+__device__ __forceinline__ void rows_sync(int w, int q) { asm volatile("bar.sync %0, 64;" ::"r"(1 + w * 4 + q) : "memory"); }  // the two of 32 rows
 __device__ __forceinline__ uint32_t low32(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }  // n low bits
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 // Pairs of fp32 values, an operation on both at once.
@@ -103,12 +109,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 // 2^y of both halves for finite y: 2^n 2^f with n the nearest whole number, found by adding 1.5 x 2^23, and the Taylor sum of
-// e^(f ln 2), |f| <= 1/2, to the power DEG: off by (ln 2 / 2)^(DEG + 1) / (DEG + 1)!, 4.2e-5, 2.4e-6 or 1.2e-7 for 4, 5, 6.
+// e^(f ln 2), |f| <= 1/2, to the power DEG: off by (ln 2 / 2)^(DEG + 1) / (DEG + 1)!, 4.2e-5 or 2.4e-6 for 4, 5.
 // Below 2^-126 the result stays there.
 template <int DEG>
 __device__ __forceinline__ void exp2_poly(uint64_t y, float &lo, float &hi) {
-    constexpr float kC[7] = {1.0f,           0.69314718056f,  0.24022650696f, 0.05550410866f,
-                             0.00961812911f, 0.00133335581f, 0.000154035304f};  // ln(2)^k / k!
+    constexpr float kC[6] = {1.0f, 0.69314718056f, 0.24022650696f, 0.05550410866f, 0.00961812911f, 0.00133335581f};  // ln(2)^k / k!
     float a, b;
     unpack2(y, a, b);
     a = fmaxf(a, -126.0f);
@@ -390,12 +395,14 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                 }
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int e = 4; e < 32; ++e) mx[e & 3] = max_nan(mx[e & 3], s[e]);
-                float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
+                for (int e = 4; e < 28; e += 8)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) mx[f] = max_nan(mx[f], s[e + f], s[e + 4 + f]);
+                float top = max_nan(max_nan(max_nan(mx[0], mx[1], s[28]), max_nan(mx[2], mx[3], s[29])), s[30], s[31]);
                 top = see ? top * scale : -INFINITY;
                 // both halves of S have been read when both maxima are there: the weights may replace any of it
                 s_top[turn][w][hf][row] = top;
-                tile_sync(w);
+                rows_sync(w, warp & 3);
                 top = max_nan(top, s_top[turn][w][hf ^ 1][row]);
                 turn ^= 1;
                 const bool plain = __all_sync(0xffffffffu, open && top < INFINITY);  // no mask, no NaN, no infinity
@@ -466,14 +473,15 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                 uint64_t sums[2] = {0, 0};
                 {
                     float *x = s;
-                    // Three pairs of eight go to a polynomial: the exponential unit alone would take 1024 cycles for a
-                    // 128 x 128 tile, as long as both products, and it serves both row tiles.
+                    // For 16-bit outputs one pair of eight goes to a polynomial: the exponential unit takes 1024 cycles for
+                    // the 256 rows of a tile otherwise, the warps' other instructions 850.  An fp32 output's terms leave no
+                    // issue slots for that.
                     if (plain) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const uint64_t y = fma2(pack2(x[2 * e], x[2 * e + 1]), scales, shift);
-                            if ((e & 7) < 3) {
-                                exp2_poly<T::TERMS == 1 ? (BF16 ? 4 : 5) : 6>(y, x[2 * e], x[2 * e + 1]);
+                            if (!F32 && (e & 7) < 1) {
+                                exp2_poly<BF16 ? 4 : 5>(y, x[2 * e], x[2 * e + 1]);
                             } else {
                                 unpack2(y, x[2 * e], x[2 * e + 1]);
                                 x[2 * e] = ex2(x[2 * e]);
@@ -487,16 +495,20 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) sums[e & 1] = add2(sums[e & 1], pack2(x[2 * e], x[2 * e + 1]));
                     }
+                    // All terms but the last are cut off, not rounded: what is left is exact, and takes one operation a pair.
 #pragma unroll
                     for (int t = 0; t < T::TERMS; ++t) {
                         uint32_t u[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            u[e] = pack16<BF16>(x[2 * e], x[2 * e + 1]);
-                            if (t + 1 < T::TERMS) {
-                                x[2 * e] -= low16<BF16>(u[e]);
-                                x[2 * e + 1] -= high16<BF16>(u[e]);
+                            if (t + 1 == T::TERMS) {
+                                u[e] = pack16<BF16>(x[2 * e], x[2 * e + 1]);
+                                continue;
                             }
+                            constexpr uint32_t kKeep = BF16 ? 0xffff0000u : 0xffffe000u;
+                            const float a = __uint_as_float(__float_as_uint(x[2 * e]) & kKeep), b = __uint_as_float(__float_as_uint(x[2 * e + 1]) & kKeep);
+                            u[e] = BF16 ? __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632) : pack16<BF16>(a, b);
+                            unpack2(fma2(pack2(a, b), pack2(-1.0f, -1.0f), pack2(x[2 * e], x[2 * e + 1])), x[2 * e], x[2 * e + 1]);
                         }
                         tmem_st16(region + hf * (16 * T::TERMS) + t * 16, u);
                     }
@@ -524,9 +536,10 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             }
             // the halves' sums meet (the maxima are the same); nobody reads the other turn's any more
             s_top[turn][w][hf][row] = l;
-            tile_sync(w);
+            rows_sync(w, warp & 3);
             if (hf == 0 && r < M) P.ml[to + row] = make_float2(m, l + s_top[turn][w][1][row]);
             turn ^= 1;
+            tile_sync(w);                   // all its warps have looked at the last tiles' values
             const int late = keys - fresh;  // new slots there are
             const unsigned long long there = late >= 64 ? ~0ull : late <= 0 ? 0ull : (1ull << late) - 1;
             const unsigned long long odd = (s_odd[0] | (unsigned long long)s_odd[1] << 32) & bits & there;
