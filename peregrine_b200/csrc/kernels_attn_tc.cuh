@@ -79,6 +79,14 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {  /
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 __device__ __forceinline__ void tile_sync(int w) { asm volatile("bar.sync %0, 256;" ::"r"(9 + w) : "memory"); }  // the warps of a row tile
+__device__ __forceinline__ bool rows_any(int w, int q, bool v) {  // the same with a vote
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %2, 0;\n\tbar.red.or.pred p, %1, 64, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(r)
+                 : "r"(1 + w * 4 + q), "r"((uint32_t)v)
+                 : "memory");
+    return r != 0;
+}
 __device__ __forceinline__ void rows_sync(int w, int q) { asm volatile("bar.sync %0, 64;" ::"r"(1 + w * 4 + q) : "memory"); }  // the two of 32 rows
 __device__ __forceinline__ uint32_t low32(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }  // n low bits
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -400,16 +408,22 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
                     for (int f = 0; f < 4; ++f) mx[f] = max_nan(mx[f], s[e + f], s[e + 4 + f]);
                 float top = max_nan(max_nan(max_nan(mx[0], mx[1], s[28]), max_nan(mx[2], mx[3], s[29])), s[30], s[31]);
                 top = see ? top * scale : -INFINITY;
-                // both halves of S have been read when both maxima are there: the weights may replace any of it
-                s_top[turn][w][hf][row] = top;
-                rows_sync(w, warp & 3);
-                top = max_nan(top, s_top[turn][w][hf ^ 1][row]);
-                turn ^= 1;
-                const bool plain = __all_sync(0xffffffffu, open && top < INFINITY);  // no mask, no NaN, no infinity
+                // The usual tile needs no more than the two threads of every row to agree that it is one: no mask, no NaN, no
+                // infinity, and no maximum that has grown too far.  (They have both read S then: weights may replace any of it.)
                 if (i) pvph ^= 1u;
-                if (i == 0) {
-                    m = top;
-                } else if (__any_sync(0xffffffffu, top > m + kAtLag)) {
+                bool plain = true, grown = false;
+                if (rows_any(w, warp & 3, i == 0 || !(open && top <= m + kAtLag))) {
+                    s_top[turn][w][hf][row] = top;
+                    rows_sync(w, warp & 3);
+                    top = max_nan(top, s_top[turn][w][hf ^ 1][row]);
+                    turn ^= 1;
+                    plain = __all_sync(0xffffffffu, open && top < INFINITY);
+                    if (i == 0)
+                        m = top;
+                    else
+                        grown = __any_sync(0xffffffffu, top > m + kAtLag);
+                }
+                if (grown) {
                     // O of this row tile is at rest: the product before was committed with these scores, or is waited for
                     if (T::BUFS > 1) {
                         um_spin(pvdone + 8 * w, pvph, fail);
