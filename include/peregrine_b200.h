@@ -264,7 +264,7 @@ typedef struct ColiCudaKv {
  * Per q and k head: y = x * rsqrt(mean(x^2) + eps) * w (q_w / k_w fp32 [D], NULL = no norm), then the first
  * R dims (even, 0 <= R <= D) turn by pos_dev[s] * theta^(-2j/R) (angles in 64 bits): style 0 takes
  * pairs (2j, 2j+1) to (j, R/2 + j) as coli_cuda_pipe_rope does, style 1 pairs (j, R/2 + j) in place.  Values
- * are stored as they are.  q_out [S, H, D] has the cache's dtype; kv->pos receives pos_dev[s] and kv->acc zero
+ * are stored as they are.  q_out [S, H, D] has the cache's dtype and lies outside qkv_dev's rows; kv->pos receives pos_dev[s] and kv->acc zero
  * at the stored slots. */
 int coli_cuda_pipe_qk_norm_rope(int device, void *q_out, const float *qkv_dev, long long row_stride, int S, int H,
                                 const ColiCudaKv *kv, const float *q_w, const float *k_w, float eps,

@@ -20,7 +20,7 @@ def view(**kw):
 
 
 def norm(kv=None, **kw):
-    a = dict(q_out=P, qkv=P, rows=4, heads=4, base=P, pos=P, theta=1e4, rotary=64, style=0, q_weight=P, k_weight=P,
+    a = dict(q_out=2 * P, qkv=P, rows=4, heads=4, base=P, pos=P, theta=1e4, rotary=64, style=0, q_weight=P, k_weight=P,
              eps=1e-6, rows_per_seq=2, row_stride=8 * 64)
     a.update(kw)
     at.qk_norm_rope(0, kv=kv or view(), **a)
@@ -81,7 +81,8 @@ def test_caches_that_do_not_hold_together(capfd, call, bad, why):
     (dict(row_stride=8 * 64 - 4), "row stride"), (dict(row_stride=1 << 41), "row stride"), (dict(rotary=63), "rotary"),
     (dict(rotary=66), "rotary"), (dict(rotary=-2), "rotary"), (dict(style=2), "style"), (dict(theta=0.0), "theta"),
     (dict(theta=float("inf")), "theta"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
-    (dict(pos=P + 2), "misaligned"), (dict(k_weight=P + 1), "misaligned")])
+    (dict(pos=P + 2), "misaligned"), (dict(k_weight=P + 1), "misaligned"), (dict(q_out=P), "overlaps"),
+    (dict(q_out=P + 4 * 512 * 4 - 16), "overlaps"), (dict(q_out=P - 4 * 4 * 64 * 2 + 16), "overlaps")])
 def test_norm_refusals(capfd, bad, why):
     err = said(capfd, norm, **bad)
     assert why in err and "not initialised" not in err

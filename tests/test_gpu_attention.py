@@ -391,6 +391,60 @@ def test_evict_caches_past_a_cluster(dev):
 
 
 # --------------------------------------------------------------------------- together, and recorded
+def test_calls_of_every_kernel_recorded_and_replayed(dev):
+    """A graph of two attention calls (many row vectors with weights, and one row a sequence) and an eviction by a cluster,
+    each with scratch of its own, replayed after the lengths, queries and weights on the device have changed: the bits of
+    the same calls made directly."""
+    L, rng = cuda.lib(), np.random.default_rng(7)
+    n, r, H, Kv, D, cap, Tp, keep = 3, 8, 12, 2, 128, 3000, 500, 900
+    k, v = (ref.cache(rng, n, Kv, cap, D, "bf16") for _ in range(2))
+    pk, pv = (ref.cache(rng, 1, Kv, Tp, D, "bf16") for _ in range(2))
+    dk, dv = (torch.zeros((n, Kv, keep, D), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pos = i32(np.broadcast_to(np.arange(cap), (n, Kv, cap)))
+    acc, dacc = torch.zeros((n, Kv, cap), device="cuda"), torch.zeros((n, Kv, keep), device="cuda")
+    dpos, index, new_len = i32(np.zeros((n, Kv, keep))), i32(np.zeros((n, Kv, keep))), i32([0] * n)
+    q, one = (torch.zeros((m, H, D), dtype=torch.bfloat16, device="cuda") for m in (n * r, n))
+    out, out1 = torch.zeros((n * r, H, D), device="cuda"), torch.zeros((n, H, D), dtype=torch.bfloat16, device="cuda")
+    base, length = i32([0] * n), i32([0] * n)
+    own, pre, to = ref.view(k, v, "bf16", pos, acc), ref.view(pk, pv, "bf16"), ref.view(dk, dv, "bf16", dpos, dacc)
+    plain = ref.view(k, v, "bf16")
+    need, need1 = at.attention_workspace(0, n * r, H, own, Tp, r), at.attention_workspace(0, n, H, plain, 0, 1)
+    work, work1 = (torch.zeros(m, dtype=torch.uint8, device="cuda") for m in (need, need1))
+    torch.cuda.synchronize()
+
+    def calls():
+        at.attention(0, out.data_ptr(), q.data_ptr(), n * r, H, own, base.data_ptr(), 0.1, work.data_ptr(), need, rows_per_seq=r,
+                     prefix=pre, prefix_len=Tp)
+        at.attention(0, out1.data_ptr(), one.data_ptr(), n, H, plain, base.data_ptr(), 0.1, work1.data_ptr(), need1,
+                     out_f32=False)
+        at.kv_evict(0, to, own, length.data_ptr(), new_len.data_ptr(), index.data_ptr(), keep, 4, 50)
+
+    handle = C.c_void_p()
+    assert L.coli_cuda_graph_begin(0) == 1
+    calls()
+    assert L.coli_cuda_graph_end(0, C.byref(handle)) == 1
+    for lens in ([1000, 64, 2992], [3, 2999, 1500], [-1, 700, 901]):
+        new_q, new_one = (torch.from_numpy(rng.standard_normal(t.shape, dtype=np.float32)) for t in (q, one))
+        start = torch.from_numpy(rng.random((n, Kv, cap), dtype=np.float32))
+        got = []
+        for graph in (True, False):
+            q.copy_(new_q), one.copy_(new_one), acc.copy_(start), base.copy_(i32(lens)), length.copy_(i32([x + r for x in lens]))
+            for t in (out, out1, dk, dv, dacc, dpos, index, new_len):
+                t.zero_()
+            torch.cuda.synchronize()
+            if graph:
+                assert L.coli_cuda_graph_launch(handle) == 1
+            else:
+                calls()
+            ref.done()
+            got.append([t.clone() for t in (out, out1, acc, dk, dv, dacc, dpos, index, new_len)])
+        for a, b in zip(*got):
+            assert torch.equal(a, b)
+        assert float(got[0][0].abs().sum()) > 0
+    L.coli_cuda_graph_free(handle)
+    assert cuda.last_device_error(0) == 0
+
+
 def test_a_decode_loop_with_all_three_recorded_as_a_graph(dev):
     """Steps of norm + store, attention with weights and (at the end) an eviction, once call by call and once as a
     graph replayed on device-side lengths: the same bits, and the attention follows the lengths of the replay."""
