@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
     const long long line_pre = (long long)nkv * P.tcm_pre * tp;
     long long first = 0, end = 0;
     int seq = 0, off = 0;
-    if (!line_share<T::THREADS / 32>(P.own.n_seq, [&](int b) { return tc_tiles(P, b); }, per_seq, line_pre, P.tc_ctas, kTcLeast, first, end, seq,
+    if (!line_share<T::THREADS / 32>(P.tc_own ? P.own.n_seq : 0, [&](int b) { return tc_tiles(P, b); }, per_seq, line_pre, P.tc_ctas, kTcLeast, first, end, seq,
                                      off))
         first = end = 0;
     TcAt at;
