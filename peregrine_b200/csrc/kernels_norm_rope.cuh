@@ -8,6 +8,8 @@
 // row's cosines is the same for all heads of the row: a warp works on a stretch of the batch's heads in order and keeps both in
 // registers; its input comes by bulk copies of up to 4 kB, one being worked on and one under way (24 warps an SM, 96 kB).
 // Frequencies (64 bits) are formed once per CTA.
+// Measured: 4096 rows of 48 + 16 heads of 128 in 43 us, 4.7 TB/s (72 % of the copy rate); about 150 instructions for a warp's
+// 256 values keep the issue slots as busy as HBM.
 // Angles are formed and reduced to turns in 64 bits: at position 10^6 an fp32 product is off by 0.03.
 #pragma once
 #include <cuda_bf16.h>
