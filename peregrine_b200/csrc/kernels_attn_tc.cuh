@@ -11,7 +11,7 @@
 // O / l.  With at most 128 row vectors both tiles hold the same ones and the key tiles go to them in turn.  D = 256 has
 // no room for a second O: there one tile alternates between two S.
 //
-// Measured: 32 rows x 64 heads behind 32768 keys (8 key heads of 128, bf16 out) 50 us, 686 TFLOP/s of the 1669 that cuBLAS
+// Measured: 32 rows x 64 heads behind 32768 keys (8 key heads of 128, bf16 out) 48 us, 716 TFLOP/s of the 1669 that cuBLAS
 // reaches; 0.77 us a step of 64 keys x 256 rows, 1430 cycles of the 1280 that the products need (a 64-column product reads
 // its operands from shared memory for 48 cycles and multiplies for 32).  A CTA's start and end take about 9 us.
 //
@@ -92,6 +92,8 @@ __device__ __forceinline__ bool rows_any(int w, int q, bool v) {  // the same wi
     return r != 0;
 }
 __device__ __forceinline__ void rows_sync(int w, int q) { asm volatile("bar.sync %0, 64;" ::"r"(1 + w * 4 + q) : "memory"); }  // the two of 32 rows
+// Swizzle of 16-byte pieces in rows of `pieces` (4 or 8) of them: eight neighbouring rows or pieces meet all banks.
+__device__ __forceinline__ int turn_at(int row, int pieces) { return pieces == 8 ? row & 7 : (row >> 1) & 3; }
 __device__ __forceinline__ uint32_t low32(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }  // n low bits
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -360,7 +362,7 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             float m = -INFINITY, l = 0.0f;
             if (mine) {
                 // D / 8 lanes read a row together; a warp brings 16 of its 32 rows
-                constexpr int LPR = D / 8, RPI = 32 / LPR, B = 16 / RPI < 8 ? 16 / RPI : 8;
+                constexpr int LPR = D / 8, RPI = 32 / LPR, B = 16 / RPI;  // loads under way together
                 const int ch = lane % LPR, rl = (row & ~31) + hf * 16 + lane / LPR;
                 uint8_t *to = base + w * T::Q_BYTES + (ch >> 3) * (128 * 128);
                 int q = r - row + rl, div = q / P.G, rem = q - div * P.G;  // row vector, its row and head
@@ -561,37 +563,42 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             const int late = keys - fresh;  // new slots there are
             const unsigned long long there = late >= 64 ? ~0ull : late <= 0 ? 0ull : (1ull << late) - 1;
             const unsigned long long odd = (s_odd[0] | (unsigned long long)s_odd[1] << 32) & bits & there;
-            // A thread has a row's dims, a store wants a row's dims in neighbouring lanes: 32 rows x 16 dims at a time turn in
-            // the shared memory of this row tile's query vectors, whose products are done.
-            uint8_t *swap = base + w * T::Q_BYTES + (warp & 7) * 2048;
-#pragma unroll 2
-            for (int d = hf * (D / 2); d < (hf + 1) * (D / 2); d += 16) {
-                float o[16];
-                if (mine) {
-                    tmem_ld16(tmem + lanes + T::O_COL + w * D + d, o);
-                    tmem_wait_ld16(o);
-                } else {
+            // A thread has a row's dims, a store wants a row's dims in neighbouring lanes: 32 rows x CW dims at a time turn in the
+            // shared memory of this row tile's query vectors, whose products are done.  Wide pieces of a row fill whole lines of
+            // the partial results (with 16 dims at a time, and 8 loads of query vectors under way, the call above took 50 us).
+            constexpr int CW = D == 64 ? 16 : 32, CL = CW / 4;  // lanes of a row
+            uint8_t *swap = base + w * T::Q_BYTES + (warp & 7) * (CW * 128);
+#pragma unroll 1
+            for (int d = hf * (D / 2); d < (hf + 1) * (D / 2); d += CW) {
+                float o[CW];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+                for (int h = 0; h < CW; h += 16) {
+                    float v[16];
+                    if (mine) {
+                        tmem_ld16(tmem + lanes + T::O_COL + w * D + d + h, v);
+                        tmem_wait_ld16(v);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[h + e] = mine ? v[e] : 0.0f;
                 }
                 for (unsigned long long q = odd; q; q &= q - 1) {
                     const uint16_t *v = P.own.v + (long long)at.seq * P.own.seq_stride + at.kvh * P.own.head_stride +
                                         ((long long)fresh + __ffsll(q) - 1) * P.own.slot_stride + d;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
+                    for (int e = 0; e < CW; ++e) {
                         const float x = from16<BF16>(v[e]);
                         if (!isfinite(x)) o[e] += x;
                     }
                 }
                 __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    *reinterpret_cast<float4 *>(swap + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                for (int e = 0; e < CL; ++e)
+                    *reinterpret_cast<float4 *>(swap + lane * (CW * 4) + ((e ^ turn_at(lane, CL)) << 4)) = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 __syncwarp();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int rr = e * 8 + (lane >> 2), ch = lane & 3;
-                    const float4 v = *reinterpret_cast<const float4 *>(swap + rr * 64 + ((ch ^ ((rr >> 1) & 3)) << 4));
+                for (int e = 0; e < CL; ++e) {
+                    const int rr = e * (32 / CL) + lane / CL, ch = lane % CL;
+                    const float4 v = *reinterpret_cast<const float4 *>(swap + rr * (CW * 4) + ((ch ^ turn_at(rr, CL)) << 4));
                     if (r - lane + rr < M) *reinterpret_cast<float4 *>(P.part + (to + (row & ~31) + rr) * D + d + ch * 4) = v;
                 }
             }

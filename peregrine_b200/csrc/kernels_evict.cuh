@@ -153,8 +153,8 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const EvictArg
 
 // The same on a cluster of C CTAs (kEvCluster, or 1 for short caches) per (sequence, kv head): every CTA keeps the keys of its
 // part of the slots in shared memory, histograms and counts are read across the cluster.  Measured for 48 times
-// up to 40000 slots: one CTA each 108 us, clusters of eight 33, of four about 46; what is left are the exchanges (about 1 us
-// each, seven of them) and the sweeps between them.
+// up to 40000 slots: one CTA each 108 us, clusters of eight 33 (the whole call 52; with clusters of four 65); what is left are the
+// exchanges (about 1 us each, seven of them) and the sweeps between them.
 constexpr int kEvCluster = 8, kEvPartThreads = 512, kEvPartMost = 32768;  // slots of a CTA at the most
 constexpr int kEvAlone = 1024;                                            // up to here one CTA is a cluster
 
