@@ -255,7 +255,7 @@ struct AttnLaunch {
         }
         // waits on the device for the end of the launches before
         const int vectors = P.S * P.H, groups = P.own.n_seq * P.own.n_kv;
-        const bool few = vectors < 4 * P.tc_ctas, many = P.tc_own;
+        const bool few = vectors < 16 * P.tc_ctas, many = P.tc_own;
         const int row_ctas = few ? vectors : (vectors + 3) / 4, chunks = P.own.acc && !many ? (P.own.cap + kAtChunk - 1) / kAtChunk : 0;
         if (!launch_early(few ? attn_join_kernel<D, BF16, 4> : attn_join_kernel<D, BF16, 1>, (unsigned)(row_ctas + chunks * groups), kAtCombine,
                           0, stream, "attention join launch", 1, true, P, RT, row_ctas, chunks))

@@ -618,67 +618,84 @@ __global__ void __launch_bounds__(kAtThreads, SplitShape<D, RT>::PER_SM)
 }
 
 // The partials of a row vector lie in up to six runs of rows of part / ml: `n` rows, `stride` apart, from row `at` on.
+// Lane j < 6 of a warp holds run j.
 struct AttnRun {
     long long at;
     int stride, n;
 };
-// Run j of row vector r (within its sequence) of a (sequence, kv head): the prefix's and the own slots' from the split kernel (0, 1),
-// the same from the tensor-memory kernel, each in up to two halves (2 to 5).
-__device__ __forceinline__ AttnRun attn_run(const AttnArgs &P, int j, int seq, int kvh, int r, int rt) {
+// Run j of row vector r (within its sequence) of a (sequence, kv head), but for the CTAs that share its unit: the prefix's and
+// the own slots' from the split kernel (0, 1), the same from the tensor-memory kernel, each in up to two halves (2 to 5).  It
+// needs no other launch's results.
+struct AttnRunOf {
+    int unit, row, stride;
+    bool there, tc;
+};
+__device__ __forceinline__ AttnRunOf attn_run_of(const AttnArgs &P, int j, int seq, int kvh, int r, int rt) {
     const int nkv = P.own.n_kv, rp = seq * P.rows * P.G + r;
-    const bool own = j == 1 || j >= 4, tc = j >= 2;
+    const bool own = j == 1 || j >= 4;
     const int q = own ? r : rp;
-    bool there;
-    int unit, row, t = rt;
-    if (!tc) {
-        const int mt = own ? P.mt_own : P.mt_pre;
-        there = own ? own_tiles(P, seq) > 0 : P.mt_pre > 0;
-        unit = (own ? nkv * P.mt_pre + seq * nkv * P.mt_own : 0) + kvh * mt + q / t;
-        row = q % t;
+    AttnRunOf R;
+    R.tc = j >= 2;
+    int t, from;  // rows of a unit that row vectors are dealt out by, first unit of the kv head
+    if (!R.tc) {
+        t = R.stride = rt;
+        R.there = own ? own_tiles(P, seq) > 0 : P.mt_pre > 0;
+        from = own ? nkv * P.mt_pre + (seq * nkv + kvh) * P.mt_own : kvh * P.mt_pre;
     } else {
         const int two = own ? P.tc2_own : P.tc2_pre;
+        R.stride = P.tc_rows;
         t = two ? 128 : P.tc_rows;
-        there = (own ? P.tc_own && own_keys(P, seq) > 0 : P.tc_pre) && (two || !(j & 1));
-        unit = (own ? nkv * P.tcm_pre + seq * nkv * P.tcm_own + kvh * P.tcm_own : kvh * P.tcm_pre) + q / t;
-        row = q % t + (j & 1) * 128;
-        t = P.tc_rows;
+        R.there = (own ? P.tc_own && own_keys(P, seq) > 0 : P.tc_pre) && (two || !(j & 1));
+        from = own ? nkv * P.tcm_pre + (seq * nkv + kvh) * P.tcm_own : kvh * P.tcm_pre;
     }
-    AttnRun R{0, t, 0};
-    if (there) {
-        const int2 ends = (tc ? P.tc_cta_of : P.cta_of)[unit];
+    R.there = R.there && j < 6;
+    const int mt = (int)((unsigned)q / (unsigned)t);
+    R.unit = from + mt;
+    R.row = q - mt * t + (R.tc && (j & 1) ? 128 : 0);
+    return R;
+}
+__device__ __forceinline__ AttnRun attn_run(const AttnArgs &P, const AttnRunOf &of) {
+    AttnRun R{0, of.stride, 0};
+    if (of.there) {
+        const int2 ends = (of.tc ? P.tc_cta_of : P.cta_of)[of.unit];
         R.n = ends.y - ends.x + 1;
-        R.at = ((long long)unit + ends.x) * t + row + (tc ? P.tc_row0 : 0);
+        R.at = ((long long)of.unit + ends.x) * of.stride + of.row + (of.tc ? P.tc_row0 : 0);
     }
     return R;
 }
-// All runs in the registers of every lane, and what the partials' statistics say: maximum and sum over all of them.
-struct AttnRow {
-    AttnRun run[6];
-    int n;
-    float m, l;
-    __device__ __forceinline__ long long at(int j) const {
-        long long r = 0;
-#pragma unroll
-        for (int k = 0; k < 6; ++k) {
-            if (j >= 0 && j < run[k].n) r = run[k].at + (long long)j * run[k].stride;
-            j -= run[k].n;
-        }
-        return r;
-    }
-};
-__device__ __forceinline__ void attn_row(const AttnArgs &P, AttnRow &R, int lane, int seq, int kvh, int r, int rt) {
-    const AttnRun mine = attn_run(P, min(lane, 5), seq, kvh, r, rt);
-    R.n = 0;
+// Row of part / ml of partial j, counted over all runs.
+__device__ __forceinline__ long long attn_partial(const AttnRun &run, int j) {
+    int in = 0, off = 0;
 #pragma unroll
     for (int k = 0; k < 6; ++k) {
-        R.run[k].at = __shfl_sync(0xffffffffu, mine.at, k);
-        R.run[k].stride = __shfl_sync(0xffffffffu, mine.stride, k);
-        R.run[k].n = __shfl_sync(0xffffffffu, mine.n, k);
-        R.n += R.run[k].n;
+        const int n = __shfl_sync(0xffffffffu, run.n, k);
+        if (j >= 0 && j < n) {
+            in = k;
+            off = j;
+        }
+        j -= n;
     }
+    const long long at = __shfl_sync(0xffffffffu, run.at, in);
+    return at + (long long)off * __shfl_sync(0xffffffffu, run.stride, in);
+}
+// What the statistics of all partials say: maximum and sum; and each lane's place among the first 32, with its maximum.
+struct AttnRow {
+    long long at;
+    int n;
+    float m, l, at_m;
+};
+__device__ __forceinline__ AttnRow attn_row(const AttnArgs &P, const AttnRun &run, int lane) {
+    AttnRow R;
+    R.n = __reduce_add_sync(0xffffffffu, lane < 6 ? run.n : 0);
     float m = -INFINITY, l = 0.0f;
-    for (int j = lane; j < R.n; j += 32) {
-        const float2 ml = P.ml[R.at(j)];
+    for (int j0 = 0; j0 < R.n || j0 == 0; j0 += 32) {
+        const long long at = attn_partial(run, j0 + lane);
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (j0 + lane < R.n) ml = P.ml[at];
+        if (j0 == 0) {
+            R.at = at;
+            R.at_m = ml.x;
+        }
         const float to = fmaxf(m, ml.x);
         if (to != -INFINITY) {
             l = l * ex2(m - to) + ml.y * ex2(ml.x - to);
@@ -696,6 +713,7 @@ __device__ __forceinline__ void attn_row(const AttnArgs &P, AttnRow &R, int lane
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     R.m = top;
     R.l = l;
+    return R;
 }
 
 // Adds the weights 2^(x - m) / l of four slots to their sums.
@@ -707,46 +725,59 @@ __device__ __forceinline__ void attn_weigh(float (&sum)[4], const float4 &x, con
 }
 
 // Joins the partials.  The first `row_ctas` CTAs take 4 / WPR row vectors each, WPR warps to one (4 where there are too few
-// row vectors to fill the device); with acc and up to kAtMany row vectors a problem, further CTAs take 1024 slots of one
-// (sequence, kv head) each.  What bounds it is the partials' way from the second-level cache (22 of 512 bytes a row vector in
-// a batch of 32 behind a prefix of 32768: 23 MB in 7 us; eight loads under way instead of one took no less).
+// row vectors to fill the device with a warp each: below 16 an SM; 24.8 instead of 29.0 us for a call of 1120 row vectors, 91.9
+// instead of 93.6 for one of 2048); with acc and up to kAtMany row vectors a problem, further CTAs take 1024 slots of one
+// (sequence, kv head) each.  What bounds it is a chain of latencies (CTAs of a unit, statistics, partials), so all that does
+// not hang on the launches before comes ahead of the wait for them, and eight partials of a warp are under way together.
 template <int D, bool BF16, int WPR>
 __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P, int rt, int row_ctas, int chunks) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    griddep_wait();
-    griddep_launch_dependents();
     if (blockIdx.x < (unsigned)row_ctas) {
         constexpr int E = D / 32;
         __shared__ float s_o[WPR][WPR == 1 ? 1 : D];
-        const int u = blockIdx.x * (4 / WPR) + warp / WPR, sub = warp % WPR;
-        if (u >= P.S * P.H) return;
-        const int row = u / P.H, h = u % P.H, seq = row / P.rows, kvh = h / P.G;
-        if (P.base[seq] < 0) return;
-        AttnRow R;
-        attn_row(P, R, lane, seq, kvh, (row % P.rows) * P.G + h % P.G, rt);
+        const unsigned u = blockIdx.x * (4 / WPR) + warp / WPR;
+        const int sub = warp % WPR;
+        // lengths came before the launches that this one waits for
+        const bool mine = u < (unsigned)(P.S * P.H);
+        const unsigned row = u / (unsigned)P.H, h = u - row * P.H, seq = row / (unsigned)P.rows, kvh = h / (unsigned)P.G;
+        const bool none = !mine || P.base[seq] < 0;
+        AttnRunOf of{};
+        if (!none) of = attn_run_of(P, lane, seq, kvh, (row - seq * P.rows) * P.G + (h - kvh * P.G), rt);
+        griddep_wait();
+        griddep_launch_dependents();
+        if (none) return;
+        const AttnRun run = attn_run(P, of);
+        const AttnRow R = attn_row(P, run, lane);
         float o[E] = {};
         for (int j0 = 0; j0 < R.n; j0 += 32) {
-            const int j = j0 + lane;
-            const long long mine = j < R.n ? R.at(j) : 0;
-            const float w = j < R.n ? ex2(P.ml[mine].x - R.m) : 0.0f;
+            const long long mine = j0 ? attn_partial(run, j0 + lane) : R.at;
+            const float w = j0 + lane < R.n ? ex2((j0 ? P.ml[mine].x : R.at_m) - R.m) : 0.0f;
             const int n = min(32, R.n - j0);
-#pragma unroll 8
-            for (int i = sub; i < n; i += WPR) {
-                const float f = __shfl_sync(0xffffffffu, w, i);
-                const float *src = P.part + __shfl_sync(0xffffffffu, mine, i) * D + lane * E;
+            constexpr int V = E < 4 ? 2 : 4, B = 8;  // floats of a load, partials under way together
+            for (int i0 = sub; i0 < n; i0 += B * WPR) {
+                float x[B][E];
 #pragma unroll
-                for (int e = 0; e < E; e += E < 4 ? 2 : 4)
-                    if (E < 4) {
-                        const float2 v = *reinterpret_cast<const float2 *>(src + e);
-                        o[e] = fmaf(v.x, f, o[e]);
-                        o[e + 1] = fmaf(v.y, f, o[e + 1]);
-                    } else {
-                        const float4 v = *reinterpret_cast<const float4 *>(src + e);
-                        o[e] = fmaf(v.x, f, o[e]);
-                        o[e + 1] = fmaf(v.y, f, o[e + 1]);
-                        o[(e + 2) % E] = fmaf(v.z, f, o[(e + 2) % E]);
-                        o[(e + 3) % E] = fmaf(v.w, f, o[(e + 3) % E]);
+                for (int k = 0; k < B; ++k) {
+                    const int i = i0 + k * WPR;
+                    const float *src = P.part + __shfl_sync(0xffffffffu, mine, i & 31) * D + lane * E;
+#pragma unroll
+                    for (int e = 0; e < E; e += V) {
+                        if (V == 2) {
+                            const float2 v = i < n ? *reinterpret_cast<const float2 *>(src + e) : make_float2(0.0f, 0.0f);
+                            x[k][e] = v.x, x[k][e + 1] = v.y;
+                        } else {
+                            const float4 v = i < n ? *reinterpret_cast<const float4 *>(src + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            x[k][e] = v.x, x[k][e + 1] = v.y, x[k][(e + 2) % E] = v.z, x[k][(e + 3) % E] = v.w;
+                        }
                     }
+                }
+#pragma unroll
+                for (int k = 0; k < B; ++k) {
+                    const int i = i0 + k * WPR;
+                    const float f = __shfl_sync(0xffffffffu, w, i & 31);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] = fmaf(x[k][e], i < n ? f : 0.0f, o[e]);
+                }
             }
         }
         if (WPR > 1) {
@@ -776,6 +807,8 @@ __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P,
         return;
     }
     // acc[slot] += sum over the group's row vectors of 2^(x - m) / l
+    griddep_wait();
+    griddep_launch_dependents();
     const int u = blockIdx.x - row_ctas, g = u / chunks, chunk = u % chunks;
     const int seq = g / P.own.n_kv, kvh = g % P.own.n_kv;
     const int keys = own_keys(P, seq);
@@ -784,8 +817,7 @@ __global__ void __launch_bounds__(kAtCombine) attn_join_kernel(const AttnArgs P,
     __shared__ float2 s_row[kAtMany];  // m and 1 / l of the row vectors
     const int M = P.rows * P.G, t0 = chunk * kAtChunk + threadIdx.x;
     for (int r = warp; r < M; r += 4) {
-        AttnRow R;
-        attn_row(P, R, lane, seq, kvh, r, rt);
+        const AttnRow R = attn_row(P, attn_run(P, attn_run_of(P, lane, seq, kvh, r, rt)), lane);
         if (lane == 0) s_row[r] = make_float2(R.m - kAtLift<BF16>, R.l == 0.0f ? 0.0f : 1.0f / R.l);
     }
     __syncthreads();

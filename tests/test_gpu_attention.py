@@ -191,6 +191,13 @@ def test_attention_many_rows_behind_a_prefix(dev, n, D, out_f32, T):
     run_attention(n, n, 1, 16, 2, D, T, 40, [(7 * b) % 40 for b in range(n)], Tp=700, out_f32=out_f32, acc=n == 16)
 
 
+@pytest.mark.parametrize("D, out_f32, T", [(64, True, "f16"), (128, False, "f16"), (128, True, "bf16"), (256, False, "bf16")])
+def test_attention_more_row_vectors_than_warps(dev, D, out_f32, T):
+    """Over 16 row vectors an SM: a warp joins one (two of one sequence's tiles and ten of the shared ones, and padding between)."""
+    run_attention(D, 41, 1, 64, 2, D, T, 140, [-1 if b == 17 else (11 * b) % 140 for b in range(41)], Tp=1500, out_f32=out_f32)
+    run_attention(D + 1, 2, 40, 32, 2, D, T, 200, [160, 3], Tp=300, out_f32=out_f32, acc=True)
+
+
 def test_attention_trees_and_rows_that_see_nothing(dev):
     rng = np.random.default_rng(5)
     bits = [int(rng.integers(0, 256)) for _ in range(24)]
