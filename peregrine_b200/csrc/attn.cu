@@ -352,7 +352,7 @@ PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, 
             return refuse("%s: the prefix is not one sequence of the cache's heads and type", what);
         if (prefix_len > prefix->cap) return refuse("%s: prefix of %d slots in a cache of %d", what, prefix_len, prefix->cap);
     }
-    if (!(scale == scale) || scale - scale != 0.0f) return refuse("%s: scale is not finite", what);
+    if (!std::isfinite(scale * 1.4426950408889634f)) return refuse("%s: scale is not finite in units of log2(e)", what);
     P.out = out_dev;
     P.out_f32 = out_f32;
     P.q = static_cast<const uint16_t *>(q_dev);
@@ -400,6 +400,21 @@ PGB_EXPORT int coli_cuda_pipe_kv_evict(int device, const ColiCudaKv *dst, const 
                         P.dst.head_stride == P.src.head_stride && P.dst.slot_stride == P.src.slot_stride;
     if (!same && (same_k || dst->v == src->v || dst->pos == src->pos || dst->acc == src->acc))
         return refuse("%s: source and target share some of their memory", what);
+    if (!same) {
+        const auto dense = [](const KvArgs &a) {
+            return a.slot_stride == a.D && (a.n_kv == 1 || a.head_stride == (long long)a.cap * a.D) &&
+                   (a.n_seq == 1 || a.seq_stride == (long long)a.n_kv * a.cap * a.D);
+        };
+        const auto meet = [&](const void *d, const void *f, size_t each) {  // blocks of `each` bytes a slot
+            const size_t slots = (size_t)src->n_seq * src->n_kv;
+            const uintptr_t a = reinterpret_cast<uintptr_t>(d), b = reinterpret_cast<uintptr_t>(f);
+            return a < b + slots * src->cap * each && b < a + slots * dst->cap * each;
+        };
+        const size_t row = (size_t)src->D * 2;
+        if (meet(dst->pos, src->pos, 4) || meet(dst->acc, src->acc, 4) || meet(dst->pos, src->acc, 4) || meet(dst->acc, src->pos, 4) ||
+            (dense(P.src) && dense(P.dst) && (meet(dst->k, src->k, row) || meet(dst->v, src->v, row) || meet(dst->k, src->v, row) || meet(dst->v, src->k, row))))
+            return refuse("%s: source and target share some of their memory", what);
+    }
     const long long groups = (long long)src->n_seq * src->n_kv;
     if (groups > 1 << 20) return refuse("%s: too many sequences and heads", what);
     P.len = len_dev;

@@ -97,7 +97,8 @@ def test_norm_refusals(capfd, bad, why):
     (dict(prefix=view(n_seq=1, cap=100, n_kv=1)), "one sequence"),
     (dict(prefix=view(n_seq=1, cap=100, dtype="f16")), "one sequence"),
     (dict(prefix=view(n_seq=1, cap=100, head_dim=128)), "one sequence"),
-    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale")])
+    (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(scale=3e38), "scale")])
 def test_attention_refusals(capfd, bad, why):
     err = said(capfd, attend, **bad)
     assert why in err and "not initialised" not in err
@@ -113,7 +114,11 @@ def test_attention_needs_no_prefix(capfd):
     (dict(index=P + 2), "misaligned"), (dict(src=view(pos=0)), "pos and acc"), (dict(src=view(acc=0)), "pos and acc"),
     (dict(src=view(n_kv=1)), "differ"), (dict(src=view(dtype="f16")), "differ"), (dict(src=view(head_dim=128)), "differ"),
     (dict(src=view(n_seq=1)), "differ"), (dict(dst=view(cap=8)), "share"),
-    (dict(dst=view(k=2 * P, v=3 * P, pos=2 * P)), "share")])
+    (dict(dst=view(k=2 * P, v=3 * P, pos=2 * P)), "share"),
+    (dict(dst=view(k=2 * P, v=3 * P, pos=P + 4 * 4 * 16 - 4, acc=3 * P, cap=8)), "share"),
+    (dict(dst=view(k=2 * P, v=3 * P, pos=2 * P, acc=P - 4 * 4 * 8 + 4, cap=8)), "share"),
+    (dict(dst=view(k=P - 4 * 8 * 64 * 2 + 16, v=3 * P, pos=2 * P, acc=3 * P, cap=8)), "share"),
+    (dict(dst=view(k=2 * P, v=P + 4096 + 4 * 16 * 64 * 2 - 16, pos=2 * P, acc=3 * P, cap=8)), "share")])
 def test_evict_refusals(capfd, bad, why):
     err = said(capfd, evict, **bad)
     assert why in err and "not initialised" not in err
