@@ -146,8 +146,9 @@ struct NormRopeLaunch {
         P.parts = (steps + P.per - 1) / P.per;
         if ((long long)S * P.parts > 0x7fffffffll) return refuse("pipe_qk_norm_rope: too many rows and heads");
         const long long need = ((long long)S * P.parts + kNrWarps - 1) / kNrWarps, most = (long long)kNrPerSm * sms;
-        if (!opt_in(norm_rope_kernel<D, BF16>, kNrSmem)) return 0;
-        return launch_early(norm_rope_kernel<D, BF16>, (unsigned)(need < most ? need : most), kNrWarps * 32, kNrSmem, stream,
+        auto kernel = P.R & 7 ? norm_rope_kernel<D, BF16, false> : norm_rope_kernel<D, BF16, true>;
+        if (!opt_in(kernel, kNrSmem)) return 0;
+        return launch_early(kernel, (unsigned)(need < most ? need : most), kNrWarps * 32, kNrSmem, stream,
                             "qk_norm_rope launch", 1, true, P);
     }
 };
