@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs P) {
     griddep_wait();
     griddep_launch_dependents();
     const int len = P.len[seq];
-    const int count = min(min(len, P.src.cap), P.keep);
-    if (kvh == 0 && chunk == 0 && threadIdx.x == 0) P.new_len[seq] = min(len, P.keep);
+    const int count = min(min(len, P.src.cap), P.keep);  // (negative for padding, which keeps its length)
+    if (kvh == 0 && chunk == 0 && threadIdx.x == 0) P.new_len[seq] = len < 0 ? len : count;
     if (len < 0) return;
     const bool in_place = P.dst.k == P.src.k;
     const int sub = threadIdx.x / LPR, l = threadIdx.x % LPR;

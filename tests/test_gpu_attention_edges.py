@@ -1,0 +1,45 @@
+"""Calls of the attention operators at the edges of what their declarations allow, each against the formula in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from peregrine_b200 import attention as at
+from tests import attention_ref as ref
+from tests.attention_ref import TYPES, i32
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------- eviction
+@pytest.mark.parametrize("cap, dst_cap, keep, lens", [
+    (100, 150, 150, [200, 150, 101, 100, 99, 1, 0, -1, -5]),  # one CTA a (sequence, head)
+    (100, 130, 101, [2147483647, 100, 40]),
+    (3000, 3600, 3500, [4000, 3300, 3000, 2999, -1]),         # a cluster each
+    (262145, 262300, 262200, [262300]),                       # longer than a cluster's shared memory
+])
+@pytest.mark.parametrize("same_len", [False, True])
+def test_evict_lengths_past_the_source_into_a_larger_target(dev, cap, dst_cap, keep, lens, same_len):
+    """A length past the source's cap counts as cap, whatever the target could take: the new length is that of the slots
+    that were stored, and behind it neither the index nor the target says anything."""
+    n, Kv, D = len(lens), 2, 64
+    rng = np.random.default_rng(cap + keep)
+    k, v = (ref.cache(rng, n, Kv, cap, D, "bf16") for _ in range(2))
+    acc = torch.from_numpy(rng.random((n, Kv, cap), dtype=np.float32)).cuda()
+    pos = i32(np.broadcast_to(np.arange(cap), (n, Kv, cap)))
+    dk, dv = (torch.full((n, Kv, dst_cap, D), 5.0, dtype=TYPES["bf16"], device="cuda") for _ in range(2))
+    dacc, dpos = torch.full((n, Kv, dst_cap), 5.0, device="cuda"), i32(np.full((n, Kv, dst_cap), 5))
+    index, length = i32(np.full((n, Kv, keep), 77)), i32(lens)
+    new = length if same_len else i32([88] * n)
+    torch.cuda.synchronize()
+    at.kv_evict(0, ref.view(dk, dv, "bf16", dpos, dacc), ref.view(k, v, "bf16", pos, acc), length.data_ptr(), new.data_ptr(),
+                index.data_ptr(), keep, 2, 3)
+    ref.done()
+    want = [x if x < 0 else min(x, cap, keep) for x in lens]
+    assert new.cpu().tolist() == want
+    for b, m in enumerate(want):
+        stored = max(m, 0)
+        if m >= 0:
+            there = torch.arange(keep, device="cuda").where(torch.arange(keep, device="cuda") < stored, -1)
+            assert torch.equal(index[b], there.int().expand(Kv, keep))  # nothing was left out
+        for t, f, rest in ((dk, k, 5.0), (dv, v, 5.0), (dacc, acc, 5.0), (dpos, pos, 5)):
+            assert torch.equal(t[b, :, :stored], f[b, :, :stored]) and bool((t[b, :, stored:] == rest).all())
