@@ -39,16 +39,18 @@ _norm = _attend = _workspace = _evict = None  # the library's functions, bound a
 
 
 def _bind():
+    """Another thread may find a function as soon as it is bound here: it gets there with its argument types."""
     global _norm, _attend, _workspace, _evict
     L = cuda.lib()
     vp, i, f, ll, sz = C.c_void_p, C.c_int, C.c_float, C.c_longlong, C.c_size_t
-    _norm, _attend = L.coli_cuda_pipe_qk_norm_rope, L.coli_cuda_pipe_attention
-    _workspace, _evict = L.coli_cuda_pipe_attention_workspace, L.coli_cuda_pipe_kv_evict
-    _norm.argtypes = [i, vp, vp, ll, i, i, vp, vp, vp, f, vp, vp, i, f, i, i]
-    _workspace.argtypes = [i, i, i, vp, i, i]
-    _workspace.restype = sz
-    _evict.argtypes = [i, vp, vp, vp, vp, vp, i, i, i]
-    _attend.argtypes = [i, vp, i, vp, i, i, vp, i, vp, vp, i, vp, f, vp, sz]
+    norm, attend = L.coli_cuda_pipe_qk_norm_rope, L.coli_cuda_pipe_attention
+    workspace, evict = L.coli_cuda_pipe_attention_workspace, L.coli_cuda_pipe_kv_evict
+    norm.argtypes = [i, vp, vp, ll, i, i, vp, vp, vp, f, vp, vp, i, f, i, i]
+    workspace.argtypes = [i, i, i, vp, i, i]
+    workspace.restype = sz
+    evict.argtypes = [i, vp, vp, vp, vp, vp, i, i, i]
+    attend.argtypes = [i, vp, i, vp, i, i, vp, i, vp, vp, i, vp, f, vp, sz]
+    _norm, _attend, _workspace, _evict = norm, attend, workspace, evict
 
 
 def qk_norm_rope(device: int, q_out: int, qkv: int, rows: int, heads: int, kv: KvView, base: int, pos: int,
