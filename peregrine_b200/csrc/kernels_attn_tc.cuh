@@ -562,7 +562,13 @@ __global__ void __launch_bounds__(TcShape<D, BF16, F32>::THREADS, 1)
             tile_sync(w);                   // all its warps have looked at the last tiles' values
             const int late = keys - fresh;  // new slots there are
             const unsigned long long there = late >= 64 ? ~0ull : late <= 0 ? 0ull : (1ull << late) - 1;
-            const unsigned long long odd = (s_odd[0] | (unsigned long long)s_odd[1] << 32) & bits & there;
+            // ... and those of them in this partial's tiles: another's infinite value times the weight zero of a partial that
+            // has seen nothing would be NaN.  The 64 new slots lie in two tiles at the most.
+            const int j0 = fresh / N - t0, first_new = N - fresh % N;  // the first one's tile of the segment, its new slots
+            const unsigned long long low = first_new >= 64 ? ~0ull : (1ull << first_new) - 1;
+            const auto of_mine = [&](int j) { return j >= 0 && j < n && (!two || (j & 1) == w); };
+            const unsigned long long here = (of_mine(j0) ? low : 0ull) | (of_mine(j0 + 1) ? ~low : 0ull);
+            const unsigned long long odd = (s_odd[0] | (unsigned long long)s_odd[1] << 32) & bits & there & here;
             // A thread has a row's dims, a store wants a row's dims in neighbouring lanes: 32 rows x CW dims at a time turn in the
             // shared memory of this row tile's query vectors, whose products are done.  Wide pieces of a row fill whole lines of
             // the partial results (with 16 dims at a time, and 8 loads of query vectors under way, the call above took 50 us).

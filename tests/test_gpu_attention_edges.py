@@ -3,9 +3,9 @@ import numpy as np
 import pytest
 import torch
 
-from peregrine_b200 import attention as at
+from peregrine_b200 import attention as at, cuda
 from tests import attention_ref as ref
-from tests.attention_ref import TYPES, i32
+from tests.attention_ref import TYPES, f64, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,42 @@ def test_evict_lengths_past_the_source_into_a_larger_target(dev, cap, dst_cap, k
             assert torch.equal(index[b], there.int().expand(Kv, keep))  # nothing was left out
         for t, f, rest in ((dk, k, 5.0), (dv, v, 5.0), (dacc, acc, 5.0), (dpos, pos, 5)):
             assert torch.equal(t[b, :, :stored], f[b, :, :stored]) and bool((t[b, :, stored:] == rest).all())
+
+
+# --------------------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("D, T, out_f32", [(64, "bf16", True), (128, "bf16", False), (128, "f16", True), (256, "f16", False)])
+def test_infinite_values_of_many_short_sequences(dev, D, T, out_f32):
+    """A CTA works on several (sequence, head) pairs in a row, most with a single tile of keys: a row that sees an infinite
+    value of its own sequence has an infinity there, and nothing of it is left for the next pair."""
+    n, r, G, Kv, cap, hidden = 90, 9, 4, 4, 40, 5
+    rng = np.random.default_rng(D)
+    H, S = G * Kv, n * r
+    q = torch.from_numpy(rng.standard_normal((S, H, D), dtype=np.float32)).to(TYPES[T]).cuda()
+    k, v = (ref.cache(rng, n, Kv, cap, D, T) for _ in range(2))
+    base = rng.integers(0, cap - r + 1, n)
+    odd = np.arange(n) % 3 != 1
+    for b in np.nonzero(odd)[0]:
+        v[b, :, base[b] + hidden, 3] = float("inf")
+        v[b, 1, base[b] + hidden, D - 2] = float("-inf")
+    clean = v.clone()
+    clean[~torch.isfinite(clean)] = 0.0
+    out = torch.zeros((S, H, D), dtype=torch.float32 if out_f32 else TYPES[T], device="cuda")
+    own, bdev = ref.view(k, v, T), i32(base)
+    need = at.attention_workspace(0, S, H, own, 0, r)
+    work = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    for _ in range(5):
+        torch.cuda.synchronize()
+        at.attention(0, out.data_ptr(), q.data_ptr(), S, H, own, bdev.data_ptr(), D ** -0.5, work.data_ptr(), need,
+                     rows_per_seq=r, out_f32=out_f32)
+        ref.done()
+        got = f64(out).reshape(n, r, Kv, G, D)
+        want, _, gam, mag = ref.attend(f64(q), f64(k), f64(clean), base, r, D ** -0.5)
+        tol = ref.bound(gam, mag, cap + 64, want, T, out_f32)
+        inf = np.zeros(got.shape)
+        inf[odd, hidden:, :, :, 3] = np.inf
+        inf[odd, hidden:, 1, :, D - 2] = -np.inf
+        seen = ~np.isfinite(inf)
+        assert np.array_equal(got[seen], inf[seen])
+        off = (np.abs(got.reshape(want.shape) - want) / tol).reshape(got.shape)[~seen]
+        assert np.all(off <= 1.0), float(np.nanmax(off))
+    assert cuda.last_device_error(0) == 0
