@@ -82,3 +82,61 @@ def test_infinite_values_of_many_short_sequences(dev, D, T, out_f32):
         off = (np.abs(got.reshape(want.shape) - want) / tol).reshape(got.shape)[~seen]
         assert np.all(off <= 1.0), float(np.nanmax(off))
     assert cuda.last_device_error(0) == 0
+
+
+def repeats(n, r, H, Kv, D, T, Tp, cap, out_f32, acc, other):
+    rng = np.random.default_rng(n + D + cap)
+    S = n * r
+    q = torch.from_numpy(rng.standard_normal((S, H, D), dtype=np.float32)).to(TYPES[T]).cuda()
+    k, v = (ref.cache(rng, n, Kv, cap, D, T) for _ in range(2))
+    pk, pv = (ref.cache(rng, 1, Kv, max(Tp, 1), D, T) for _ in range(2))
+    base = rng.integers((cap - r) // 2, cap - r + 1, n)
+    start = torch.from_numpy(rng.random((n, Kv, cap), dtype=np.float32)).cuda()
+    a, bdev = start.clone(), i32(base)
+    out = torch.zeros((S, H, D), dtype=torch.float32 if out_f32 else TYPES[T], device="cuda")
+    own, pre = ref.view(k, v, T, acc=a if acc else None), ref.view(pk, pv, T)
+    need = at.attention_workspace(0, S, H, own, Tp, r)
+    work, first = torch.zeros(need, dtype=torch.uint8, device="cuda"), None
+    for fill in (0, 255, 63):
+        work.fill_(fill), other.fill_(fill), a.copy_(start), out.fill_(1000.0)
+        torch.cuda.synchronize()
+        at.attention(0, out.data_ptr(), q.data_ptr(), S, H, own, bdev.data_ptr(), D ** -0.5, work.data_ptr(), need,
+                     rows_per_seq=r, prefix=pre if Tp else None, prefix_len=Tp, out_f32=out_f32)
+        ref.done()
+        got = out.view(torch.int32 if out_f32 else torch.int16).clone(), a.view(torch.int32).clone()
+        assert bool((out.abs() < 100.0).all())  # all of it was written, and is finite
+        assert torch.equal(got[0], (first or got)[0]) and torch.equal(got[1], (first or got)[1]), (n, r, H, Kv, D, T, Tp, cap)
+        first = first or got
+    assert acc != torch.equal(a, start)
+    assert cuda.last_device_error(0) == 0
+
+
+@pytest.fixture(scope="module")
+def other():
+    """Memory of more than the last cache's size: filled, it leaves nothing of a call's there."""
+    return torch.zeros(1 << 28, dtype=torch.uint8, device="cuda")
+
+
+@pytest.mark.parametrize("n, r, H, Kv, D, T, Tp, cap, out_f32, acc", [
+    (1, 1, 4, 2, 64, "bf16", 0, 20000, True, True),       # one line of tiles over many CTAs
+    (3, 1, 8, 2, 128, "f16", 70, 900, False, False),
+    (2, 4, 6, 2, 256, "bf16", 129, 500, True, True),      # 12 row vectors a problem
+    (9, 1, 24, 2, 64, "f16", 1500, 400, True, True),      # the prefix on tensor memory, own slots not
+    (41, 1, 64, 2, 128, "bf16", 700, 140, False, True),   # a warp joins a row vector
+    (2, 40, 32, 2, 64, "bf16", 300, 800, True, True),     # all on tensor memory, weights of many row vectors
+    (5, 9, 16, 4, 256, "f16", 0, 300, False, False),
+])
+def test_attention_repeats_its_bits(dev, other, n, r, H, Kv, D, T, Tp, cap, out_f32, acc):
+    """The same bits from the same inputs, whatever output, scratch and the chip's caches held before."""
+    repeats(n, r, H, Kv, D, T, Tp, cap, out_f32, acc, other)
+
+
+@pytest.mark.parametrize("D, T", [(64, "bf16"), (64, "f16"), (128, "bf16"), (128, "f16"), (256, "bf16"), (256, "f16")])
+def test_attention_repeats_its_bits_over_its_ranges(dev, other, D, T):
+    rng = np.random.default_rng(D + len(T))
+    for t in range(24):
+        n, r = [(int(rng.integers(1, 40)), 1), (int(rng.integers(1, 6)), int(rng.integers(2, 17))),
+                (1, int(rng.integers(17, 65)))][t % 3]
+        Kv = int(rng.integers(1, 4))
+        Tp, cap = (int(np.exp(rng.uniform(0, np.log(2000)))) for _ in range(2))
+        repeats(n, r, Kv * int(rng.integers(1, 11)), Kv, D, T, Tp * (t & 1), cap + r, t % 4 < 2, t % 5 < 3, other)
