@@ -279,9 +279,9 @@ int coli_cuda_pipe_qk_norm_rope(int device, void *q_out, const float *qkv_dev, l
  * past own->cap.  out [S, H, D] = softmax(scale q.k) v over what the row sees, fp32 (out_f32 = 1) or the cache's
  * dtype (0); a row that sees nothing is 0; rows of a sequence with base_dev[b] < 0 are left as they were.
  * When own->acc is set, acc[b, kv head, slot] grows by the softmax weights the slot received from the rows and
- * heads of its group.  Products of 16-bit values are summed in fp32, softmax statistics are fp32, and with
- * out_f32 the weights enter the second product with at least 22 bits (the dtype's own precision otherwise).
- * Results do not change from run to run.  work_dev: scratch of the caller's, at least
+ * heads of its group.  Products of 16-bit values are summed in fp32, softmax statistics are fp32.  With out_f32 a
+ * weight w enters the second product within 2^-21 w; from an f16 cache within 2^-30 of the row's largest weight where
+ * that is more.  Without, it is rounded to the dtype (half a step, and 5e-5 w for the exponential).  Results do not change from run to run.  work_dev: scratch of the caller's, at least
  * coli_cuda_pipe_attention_workspace(...) bytes, 256-byte aligned; calls that may overlap on the GPU need one each. */
 int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, const void *q_dev, int S, int H,
                              const ColiCudaKv *prefix, int prefix_len, const ColiCudaKv *own, const int *base_dev,

@@ -110,8 +110,11 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
 }
 
 // Weights enter the second product in 16-bit terms.  A 16-bit output needs one (its own rounding is as large).  An fp32
-// output takes as many as give it 22 bits: two of f16, three of bf16.  f16 weights are scaled by 2^6 against underflow of
-// their lower term (below 2^-24): with the 2^8 that the maximum may lag behind they stay below 2^15; l carries the same factor, so it cancels.
+// output takes two of f16 or three of bf16.  Rounded to nearest these leave 2^-22 or 2^-24 of a weight, cut off (as the
+// tensor-memory kernel does) 2^-21 or 2^-22.  f16 weights are scaled by 2^6 against underflow of their lower term: its steps of
+// 2^-24 leave up to 2^-31 of the largest weight, or 2^-30 where a first term below 2^-14 was rounded too.  With the 2^8 that
+// the maximum may lag behind, weights stay below 2^15; l carries the same factor, so it cancels.  More of one is less of the other: with 2^10 and
+// 2^5 (2^-34 of the largest) an f16 batch of 32 x 64 heads behind 32768 keys took 100.1 us, with 2^13 and 2^2 106.3, with these 96.2.
 template <bool BF16>
 constexpr float kAtLift = BF16 ? 0.0f : 6.0f;
 constexpr float kAtLag = 8.0f;  // log2 by which a row's maximum may grow before o, l and m are rescaled

@@ -140,3 +140,41 @@ def test_attention_repeats_its_bits_over_its_ranges(dev, other, D, T):
         Kv = int(rng.integers(1, 4))
         Tp, cap = (int(np.exp(rng.uniform(0, np.log(2000)))) for _ in range(2))
         repeats(n, r, Kv * int(rng.integers(1, 11)), Kv, D, T, Tp * (t & 1), cap + r, t % 4 < 2, t % 5 < 3, other)
+
+
+@pytest.mark.parametrize("G, r, Tp", [(4, 1, 0), (3, 4, 0), (16, 1, 700), (4, 9, 0), (20, 1, 500)])
+@pytest.mark.parametrize("T", ["f16", "bf16"])
+def test_small_weights_beside_a_large_one(dev, T, G, r, Tp):
+    """One key takes most of the weight, 12000 others the same small share w each: what the rounding of w to 16-bit terms
+    loses is lost 12000 times over.  With an fp32 output that is up to 2^-21 w, and from an f16 cache 2^-30 of the
+    largest weight besides (f16's smallest step, behind the factor 2^6)."""
+    D, cap = 64, 12000
+    rng = np.random.default_rng(G)
+    k = torch.zeros((1, 1, cap, D), dtype=TYPES[T], device="cuda")
+    k[..., 0] = -1.0
+    k[:, :, 7, 0] = 0.0
+    v = torch.from_numpy(rng.random((1, 1, cap, D), dtype=np.float32) + 0.5).to(TYPES[T]).cuda()
+    v[..., ::2], v[:, :, 7] = 1.0, 0.0
+    pk, pv = k[:, :, 50:50 + max(Tp, 1)].contiguous(), v[:, :, 50:50 + max(Tp, 1)].contiguous()
+    base, scale = cap - r, np.float32(np.log(2.0))
+    own, pre, bdev = ref.view(k, v, T), ref.view(pk, pv, T), i32([base])
+    need = at.attention_workspace(0, r, G, own, Tp, r)
+    work = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    q, out = torch.zeros((r, G, D), dtype=TYPES[T], device="cuda"), torch.zeros((r, G, D), device="cuda")
+    sums = np.cumsum(f64(v)[0, 0], 0)[base:] + (f64(pv)[0, 0].sum(0) if Tp else 0.0)  # of the values row i sees
+    count = base + np.arange(r)[:, None] + (Tp if Tp else 0)                          # small weights row i sees
+    for x in np.linspace(6.0, 24.0, 73):
+        q[..., 0] = float(x)
+        torch.cuda.synchronize()
+        at.attention(0, out.data_ptr(), q.data_ptr(), r, G, own, bdev.data_ptr(), float(scale), work.data_ptr(), need,
+                     rows_per_seq=r, prefix=pre if Tp else None, prefix_len=Tp)
+        ref.done()
+        w = np.exp(-float(q[0, 0, 0]) * float(scale))
+        want = (w * sums / (1.0 + w * count))[:, None, :]
+        # Scores are one product each: two roundings of the scale and two of a score of up to 24 (half a step of 2^-19), to
+        # base e; 2^-22 of the exponential; both for weight and sum.  A CTA has up to 4 tiles here, 48 matrix
+        # instructions that add to a sum, two fp32 roundings each; up to 148 partial results follow.
+        each = 2 * (np.log(2.0) * (24 * 2.0 ** -23 + 2.0 ** -19) + 2.0 ** -22) + 48 * 2.0 ** -23 + 148 * 2.0 ** -24
+        tiny = 1.5 * count[:, :, None] * 2.0 ** -30 if T == "f16" else 0.0
+        off = np.abs(f64(out) - want)
+        assert np.all(off <= want * (each + 2.0 ** -21) + tiny), (x, float((off / want).max()))
