@@ -66,6 +66,17 @@ int rows_ok(int S, int H, const KvArgs &kv, int rows_per_seq, const char *what) 
     return 1;
 }
 
+// What a call of the attention and the question for its scratch have in common.
+int attn_ok(int S, int H, const KvArgs &own, int prefix_len, int rows_per_seq, const char *what) {
+    if (!rows_ok(S, H, own, rows_per_seq, what)) return 0;
+    if (rows_per_seq > 64) return refuse("%s: %d rows of a sequence are more than 64", what, rows_per_seq);
+    if (H % own.n_kv) return refuse("%s: %d heads are no multiple of %d", what, H, own.n_kv);
+    if (prefix_len < 0) return refuse("%s: negative prefix", what);
+    if ((long long)S * H > 0x3fffffff || (own.acc && ((long long)own.cap / 32 + 1) * own.n_seq * own.n_kv > 0x3fffffff))
+        return refuse("%s: too many rows and heads", what);
+    return 1;
+}
+
 template <typename F>
 int by_type(int D, int dtype, F &&f) {  // f.template operator()<D, BF16>()
     if (dtype == 1) {
@@ -322,8 +333,7 @@ PGB_EXPORT size_t coli_cuda_pipe_attention_workspace(int device, int S, int H, c
     const char *what = "pipe_attention_workspace";
     CtxRef c;
     KvArgs kv;
-    if (!kv_args(&kv, own, what) || !rows_ok(S, H, kv, rows_per_seq, what)) return 0;
-    if (prefix_len < 0 || H % kv.n_kv || rows_per_seq > 64) return (size_t)refuse("%s: shape", what);
+    if (!kv_args(&kv, own, what) || !attn_ok(S, H, kv, prefix_len, rows_per_seq, what)) return 0;
     if (!ctx_of(device, &c)) return (size_t)refuse("%s: device %d is not initialised", what, device);
     AttnArgs P{};
     const size_t need = attn_plan(&P, kv, S, H, prefix_len, rows_per_seq, c.sms, nullptr);
@@ -337,16 +347,11 @@ PGB_EXPORT int coli_cuda_pipe_attention(int device, void *out_dev, int out_f32, 
     const char *what = "pipe_attention";
     CtxRef c;
     AttnArgs P{};
-    if (!kv_args(&P.own, own, what) || !rows_ok(S, H, P.own, rows_per_seq, what)) return 0;
-    if (rows_per_seq > 64) return refuse("%s: %d rows of a sequence are more than 64", what, rows_per_seq);
-    if (H % own->n_kv) return refuse("%s: %d heads are no multiple of %d", what, H, own->n_kv);
-    if ((long long)S * H > 0x3fffffff || (own->acc && ((long long)own->cap / 32 + 1) * own->n_seq * own->n_kv > 0x3fffffff))
-        return refuse("%s: too many rows and heads", what);
+    if (!kv_args(&P.own, own, what) || !attn_ok(S, H, P.own, prefix_len, rows_per_seq, what)) return 0;
     if (!out_dev || !q_dev || !base_dev || !work_dev) return refuse("%s: null pointer", what);
     if (!aligned(out_dev, 16) || !aligned(q_dev, 16) || !aligned(base_dev, 4) || !aligned(mask_dev, 8) || !aligned(work_dev, 256))
         return refuse("%s: misaligned pointer", what);
     if (out_f32 != 0 && out_f32 != 1) return refuse("%s: out_f32 is not 0 or 1", what);
-    if (prefix_len < 0) return refuse("%s: negative prefix", what);
     if (prefix_len) {
         if (!kv_args(&P.pre, prefix, what)) return 0;
         if (prefix->n_seq != 1 || prefix->n_kv != own->n_kv || prefix->D != own->D || prefix->dtype != own->dtype)

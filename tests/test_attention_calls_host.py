@@ -1,5 +1,9 @@
 """Host side of the attention entry points: the binding, and checks that come before the device is touched."""
+import pytest
+
 from peregrine_b200 import attention as at, cuda
+
+P = 1 << 20  # an aligned address that nothing reads
 
 
 class Function:
@@ -30,3 +34,26 @@ def test_a_bound_function_is_complete_when_it_becomes_visible(monkeypatch):
     for f, args in ((at._norm, 16), (at._attend, 15), (at._workspace, 6), (at._evict, 9)):
         assert len(f.argtypes) == args
     assert at._workspace.restype is not None
+
+
+def refused(capfd, call, *a, **kw):
+    """What a call says that fails for lack of a device at the latest."""
+    assert cuda.device_count() == 0
+    with pytest.raises(cuda.CudaError):
+        call(*a, **kw)
+    return capfd.readouterr().err
+
+
+# sequences, heads, kv heads, slots, whether weights are kept, prefix
+@pytest.mark.parametrize("n, H, Kv, cap, acc, Tp", [
+    (20000, 65536, 64, 16, False, 0), (16384, 65536, 64, 16, False, 0),      # row vectors
+    (4096, 512, 256, 40000, True, 0),                                          # slots whose weights are added up
+    (1, 64, 1, 2147483647, False, 0), (100, 64, 64, 1073741824, False, 100),  # tiles
+    (2, 7, 2, 16, False, 0), (2, 8, 2, 16, False, -1),
+])
+def test_a_refused_shape_has_no_workspace(capfd, n, H, Kv, cap, acc, Tp):
+    own = at.KvView(P, 2 * P, n, Kv, cap, 64, acc=P if acc else 0, strides=(64, 64, 64))
+    pre = at.KvView(P, 2 * P, 1, Kv, 128, 64)
+    call = refused(capfd, at.attention, 0, P, P, n, H, own, P, 0.1, P, 1 << 60, prefix=pre if Tp else None, prefix_len=Tp)
+    space = refused(capfd, at.attention_workspace, 0, n, H, own, Tp)
+    assert call.split(": ", 1)[1] == space.split(": ", 1)[1]
