@@ -302,8 +302,10 @@ PGB_EXPORT int coli_cuda_pipe_qk_norm_rope(int device, void *q_out, const float 
     if (!aligned(q_out, 16) || !aligned(qkv_dev, 16) || (row_stride & 3)) return refuse("%s: rows not aligned to 16 bytes", what);
     if (!aligned(q_w, 4) || !aligned(k_w, 4) || !aligned(pos_dev, 4) || !aligned(base_dev, 4)) return refuse("%s: misaligned pointer", what);
     if (row_stride < ((long long)H + 2ll * kv->n_kv) * kv->D || row_stride > (1ll << 40)) return refuse("%s: row stride %lld is too small or large", what, row_stride);
-    const uintptr_t q0 = reinterpret_cast<uintptr_t>(q_out), x0 = reinterpret_cast<uintptr_t>(qkv_dev);
-    if (q0 < x0 + (uintptr_t)S * row_stride * 4 && x0 < q0 + (uintptr_t)S * H * kv->D * 2) return refuse("%s: q_out overlaps the rows", what);
+    if (row_stride > (1ll << 60) / S) return refuse("%s: row stride %lld is too large for %d rows", what, row_stride, S);
+    const uintptr_t q0 = reinterpret_cast<uintptr_t>(q_out), x0 = reinterpret_cast<uintptr_t>(qkv_dev),
+                    x_bytes = ((uintptr_t)(S - 1) * row_stride + ((uintptr_t)H + 2ull * kv->n_kv) * kv->D) * 4;  // to the last row's last value
+    if (q0 < x0 + x_bytes && x0 < q0 + (uintptr_t)S * H * kv->D * 2) return refuse("%s: q_out overlaps the rows", what);
     if (R < 0 || R > kv->D || (R & 1)) return refuse("%s: rotary width %d is not an even number up to %d", what, R, kv->D);
     if (style != 0 && style != 1) return refuse("%s: style %d is not 0 or 1", what, style);
     if (R && !(theta > 0.0f && theta < 3e38f)) return refuse("%s: theta must be positive", what);

@@ -57,3 +57,15 @@ def test_a_refused_shape_has_no_workspace(capfd, n, H, Kv, cap, acc, Tp):
     call = refused(capfd, at.attention, 0, P, P, n, H, own, P, 0.1, P, 1 << 60, prefix=pre if Tp else None, prefix_len=Tp)
     space = refused(capfd, at.attention_workspace, 0, n, H, own, Tp)
     assert call.split(": ", 1)[1] == space.split(": ", 1)[1]
+
+
+@pytest.mark.parametrize("rows, stride, at_byte, why", [
+    (4, 600, (3 * 600 + 512) * 4, "not initialised"),      # right behind the last row's values, before its stride ends
+    (1, 1 << 20, 512 * 4, "not initialised"),
+    (4, 600, (3 * 600 + 512) * 4 - 16, "overlaps"), (1, 1 << 20, 512 * 4 - 16, "overlaps"),
+    (4, 600, -4 * 4 * 64 * 2, "not initialised"), (4, 600, -4 * 4 * 64 * 2 + 16, "overlaps"),
+    (2147483647, 1 << 40, 0, "too large"),                 # (the rows' bytes pass 64 bits)
+])
+def test_queries_lie_outside_the_rows_and_not_their_padding(capfd, rows, stride, at_byte, why):
+    kv = at.KvView(1 << 30, 1 << 31, rows, 2, 16, 64)
+    assert why in refused(capfd, at.qk_norm_rope, 0, P + at_byte, P, rows, 4, kv, P, P, 1e4, row_stride=stride)
