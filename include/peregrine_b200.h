@@ -296,8 +296,9 @@ size_t coli_cuda_pipe_attention_workspace(int device, int S, int H, const ColiCu
  * Rank: first the protected slots, pos < sinks or pos > last - recent with last the largest position in use;
  * then by acc, larger first (NaN last, +0 = -0); ties to the lower slot.  Kept slots below min(keep, len) stay
  * where they are, and the m-th slot below it that is not kept receives the m-th kept slot from behind: no order
- * beyond that.  dst may be src itself, which then moves only the latter; else no memory of dst is src's.  index_dev [n_seq, n_kv, keep]: the
- * source slot of every kept one, -1 behind them.  new_len_dev[b] = min(len_dev[b], src->cap, keep), the slots that were
+ * beyond that.  dst may be src itself, which then moves only the latter; else no memory of dst's four arrays is src's
+ * (rows of the one may lie between rows of the other).  index_dev [n_seq, n_kv, keep]: the source slot of every kept one,
+ * -1 behind them.  new_len_dev[b] = min(len_dev[b], src->cap, keep), the slots that were
  * kept (may be len_dev itself).  Sequences with len_dev[b] < 0 are padding: nothing of them but new_len_dev[b]
  * (= len_dev[b]) is written. */
 int coli_cuda_pipe_kv_evict(int device, const ColiCudaKv *dst, const ColiCudaKv *src, const int *len_dev,

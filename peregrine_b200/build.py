@@ -17,7 +17,7 @@ SOURCES = {
                    "kernels_decode.cuh", "kernels_block.cuh", "kernels_ep.cuh", "backend_ep.inc", "w4_layout.h",
                    "expert_route.h", "w4_host.h", "backend_layer.inc", "backend_pipe.inc", "backend_noalloc.inc", "ctx.h",
                    _HEADER],
-    "attn.cu": ["ptx.cuh", "ctx.h", "kernels_norm_rope.cuh", "kernels_attn.cuh", "kernels_attn_tc.cuh", "kernels_evict.cuh", _HEADER],
+    "attn.cu": ["ptx.cuh", "ctx.h", "kernels_norm_rope.cuh", "kernels_attn.cuh", "kernels_attn_tc.cuh", "kernels_evict.cuh", "kv_overlap.h", _HEADER],
     "w4_host.cpp": ["w4_host.h", "w4_layout.h"],
 }
 

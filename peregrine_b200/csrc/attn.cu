@@ -12,6 +12,7 @@
 #include "kernels_attn_tc.cuh"
 #include "kernels_evict.cuh"
 #include "kernels_norm_rope.cuh"
+#include "kv_overlap.h"
 
 using namespace pgb;
 
@@ -409,19 +410,17 @@ PGB_EXPORT int coli_cuda_pipe_kv_evict(int device, const ColiCudaKv *dst, const 
     if (!same && (same_k || dst->v == src->v || dst->pos == src->pos || dst->acc == src->acc))
         return refuse("%s: source and target share some of their memory", what);
     if (!same) {
-        const auto dense = [](const KvArgs &a) {
-            return a.slot_stride == a.D && (a.n_kv == 1 || a.head_stride == (long long)a.cap * a.D) &&
-                   (a.n_seq == 1 || a.seq_stride == (long long)a.n_kv * a.cap * a.D);
+        const auto all = [](const KvArgs &a, Rows *r) {
+            for (const void *p : {a.k, a.v})
+                *r++ = {addr(p), (Wide)a.seq_stride * 2, (Wide)a.head_stride * 2, (Wide)a.slot_stride * 2, a.n_seq, a.n_kv, a.cap, a.D * 2};
+            for (const void *p : {(const void *)a.pos, (const void *)a.acc}) *r++ = {addr(p), 0, 0, 0, 1, 1, 1, (Wide)a.n_seq * a.n_kv * a.cap * 4};
         };
-        const auto meet = [&](const void *d, const void *f, size_t each) {  // blocks of `each` bytes a slot
-            const size_t slots = (size_t)src->n_seq * src->n_kv;
-            const uintptr_t a = reinterpret_cast<uintptr_t>(d), b = reinterpret_cast<uintptr_t>(f);
-            return a < b + slots * src->cap * each && b < a + slots * dst->cap * each;
-        };
-        const size_t row = (size_t)src->D * 2;
-        if (meet(dst->pos, src->pos, 4) || meet(dst->acc, src->acc, 4) || meet(dst->pos, src->acc, 4) || meet(dst->acc, src->pos, 4) ||
-            (dense(P.src) && dense(P.dst) && (meet(dst->k, src->k, row) || meet(dst->v, src->v, row) || meet(dst->k, src->v, row) || meet(dst->v, src->k, row))))
-            return refuse("%s: source and target share some of their memory", what);
+        Rows to[4], from[4];
+        all(P.dst, to);
+        all(P.src, from);
+        for (const Rows &d : to)
+            for (const Rows &f : from)
+                if (rows_meet(d, f)) return refuse("%s: source and target share some of their memory", what);
     }
     const long long groups = (long long)src->n_seq * src->n_kv;
     if (groups > 1 << 20) return refuse("%s: too many sequences and heads", what);
