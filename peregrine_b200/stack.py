@@ -139,7 +139,7 @@ class DeviceStack:
             raise ValueError("stack: attention is needed in every layer or in none")
         if not st.attn and (prefix_cap or budget is not None):
             raise ValueError("stack: a prefix or a budget needs attention layers")
-        if budget is not None and (budget < 1 or slack < 1 or recent > budget):
+        if budget is not None and (budget < 1 or slack < 1 or not 0 <= recent <= budget):
             raise ValueError("stack: budget and slack must be positive, and hold the recent slots")
         L = cuda.lib()
         self.device, self.st, self.batch, self.max_steps, self.ep = device, st, batch, max_steps, ep

@@ -2,6 +2,7 @@
 import pytest
 
 from peregrine_b200 import attention as at, cuda
+from peregrine_b200.stack import DeviceStack, synth_stack
 
 P = 1 << 20  # an aligned address that nothing reads
 
@@ -145,3 +146,11 @@ def test_many_sequences_in_one_allocation(capfd):
     src, dst = (at.KvView(M + 2 * f, M + (1 << 40) + 2 * f, 4096, 1, 16, 64, pos=(1 << 50) + f * n, acc=(1 << 51) + f * n,
                           strides=(128, 0, 1 << 20)) for f in (0, 64))
     assert "share" in evict(capfd, dst, src)
+
+
+@pytest.mark.parametrize("kw", [dict(budget=4, recent=-1), dict(budget=4, recent=5), dict(budget=0), dict(budget=4, slack=0)])
+def test_a_stack_refuses_a_budget_that_no_eviction_can_keep(kw):
+    st = synth_stack(seed=3, hidden=64, inter=32, dense_inter=64, n_experts=2, k=1, n_layers=1, first_dense=1, vocab=32,
+                     attention_heads=(2, 1, 64))
+    with pytest.raises(ValueError):
+        DeviceStack(0, st, 1, 4, **kw)
