@@ -45,29 +45,62 @@ def _stale(target: str, inputs) -> bool:
     return any(os.path.getmtime(p) > t for p in inputs)
 
 
+def _stamp(target: str) -> str:
+    return os.path.join(HERE, "build", os.path.basename(target) + ".cmd")
+
+
+def _command(target: str):
+    """What ``target`` was made by, or None."""
+    try:
+        with open(_stamp(target)) as f:
+            return f.read()
+    except FileNotFoundError:
+        return None
+
+
+def _remember(target: str, command: str) -> None:
+    with open(_stamp(target), "w") as f:
+        f.write(command)
+
+
+def _forget(target: str) -> None:
+    for p in (_stamp(target), target):
+        if os.path.exists(p):
+            os.remove(p)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compiles the translation units that are out of date, side by side, and links them."""
-    files = [os.path.join(CSRC, f) for s, deps in SOURCES.items() for f in [s] + deps]
-    if not (force or _stale(LIB, files)):
-        return LIB
+    """Compiles the translation units that are out of date, side by side, and links them.  A unit is so when a file of its is newer
+    or when it was compiled by another command; ``verbose`` compiles all of them, to print what each kernel takes."""
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    objs, jobs = [], []
+    stale = []
     for src, deps in SOURCES.items():
         obj = os.path.join(objdir, src + ".o")
-        objs.append(obj)
-        if force or _stale(obj, [os.path.join(CSRC, f) for f in [src] + deps]):
-            cmd = [_nvcc()] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", obj, src]
-            jobs.append((cmd, obj, subprocess.Popen(cmd, cwd=CSRC)))
+        command = " ".join(NVCC_FLAGS + ["-c", src])
+        if force or verbose or _stale(obj, [os.path.join(CSRC, f) for f in [src] + deps]) or _command(obj) != command:
+            stale.append((src, obj, command))
+    objs = [os.path.join(objdir, src + ".o") for src in SOURCES]
+    link = " ".join(LINK_FLAGS)
+    if not stale and not _stale(LIB, objs) and _command(LIB) == link:
+        return LIB
+    nvcc = _nvcc()
+    jobs = []
+    for src, obj, command in stale:
+        _forget(obj)
+        cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", "-o", obj, src]
+        jobs.append((cmd, obj, command, subprocess.Popen(cmd, cwd=CSRC)))
     failed = None
-    for cmd, obj, job in jobs:
-        if job.wait() != 0:
+    for cmd, obj, command, job in jobs:
+        if job.wait() == 0:
+            _remember(obj, command)
+        else:
             failed = subprocess.CalledProcessError(job.returncode, cmd)
-            if os.path.exists(obj):
-                os.remove(obj)
     if failed:
         raise failed
-    subprocess.check_call([_nvcc()] + LINK_FLAGS + ["-o", LIB] + objs, cwd=CSRC)
+    subprocess.check_call([nvcc] + LINK_FLAGS + ["-o", LIB + ".new"] + objs, cwd=CSRC)
+    os.replace(LIB + ".new", LIB)  # a process that has the old one loaded keeps it
+    _remember(LIB, link)
     return LIB
 
 
