@@ -377,6 +377,9 @@ int coli_cuda_last_device_error(int device);
 int coli_cuda_selftest_bounded_wait(int device, long long limit_cycles);
 /* Number of this library's kernels launched since init (all devices). */
 uint64_t coli_cuda_kernel_launches(void);
+/* Grows whenever a scratch buffer of the context has moved.  A graph recorded from calls that use it (pipe_gemm, layers)
+ * holds its addresses: it may be replayed as long as this is what it was when the recording ended. */
+uint64_t coli_cuda_scratch_generation(int device);
 /* The context's stream as a cudaStream_t, for callers that order their own work. */
 void *coli_cuda_stream(int device);
 

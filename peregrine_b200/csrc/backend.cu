@@ -334,6 +334,10 @@ PGB_EXPORT int coli_cuda_selftest_bounded_wait(int device, long long limit_cycle
            cuda_ok(cudaStreamSynchronize(c->stream), "bounded-wait self-test synchronise");
 }
 PGB_EXPORT uint64_t coli_cuda_kernel_launches(void) { return g_launches.load(); }
+PGB_EXPORT uint64_t coli_cuda_scratch_generation(int device) {
+    Ctx *c = find_ctx(device);
+    return c ? c->scratch_gen : 0;
+}
 PGB_EXPORT void *coli_cuda_stream(int device) {
     Ctx *c = find_ctx(device);
     return c ? (void *)c->stream : nullptr;

@@ -51,7 +51,7 @@ SYMBOLS = [
     "coli_cuda_moe_layer_ep_forward_dev", "coli_cuda_moe_layer_set_profile", "coli_cuda_moe_layer_profile",
     "coli_cuda_pipe_gemm_noalloc", "coli_cuda_pipe_embed", "coli_cuda_pipe_argmax",
     "coli_cuda_pipe_qk_norm_rope", "coli_cuda_pipe_attention", "coli_cuda_pipe_attention_workspace",
-    "coli_cuda_pipe_kv_evict", "coli_cuda_last_device_error", "coli_cuda_selftest_bounded_wait", "coli_cuda_kernel_launches", "coli_cuda_stream",
+    "coli_cuda_pipe_kv_evict", "coli_cuda_last_device_error", "coli_cuda_selftest_bounded_wait", "coli_cuda_kernel_launches", "coli_cuda_scratch_generation", "coli_cuda_stream",
 ]
 
 
@@ -161,6 +161,8 @@ def lib():
         L.coli_cuda_last_device_error.argtypes = [i]
         L.coli_cuda_selftest_bounded_wait.argtypes = [i, C.c_longlong]
         L.coli_cuda_kernel_launches.restype = u64
+        L.coli_cuda_scratch_generation.argtypes = [i]
+        L.coli_cuda_scratch_generation.restype = u64
         L.coli_cuda_stream.argtypes = [i]
         L.coli_cuda_stream.restype = vp
         _lib = L

@@ -355,7 +355,7 @@ class DeviceStack:
                     L.coli_cuda_graph_free(h)
                 return False
             graphs.append(g)
-        self.graphs = graphs
+        self.graphs, self._graphs_gen = graphs, L.coli_cuda_scratch_generation(dev)
         return True
 
     def run(self, steps: int):
@@ -366,6 +366,8 @@ class DeviceStack:
             return
         L, dev, b = self._L, self.device, self.batch
         vp = C.c_void_p
+        if self.graphs and self._graphs_gen != L.coli_cuda_scratch_generation(dev):
+            self._drop_graphs()  # a wider call has moved the scratch that they hold the addresses of
         if self.graphs is None:
             self.step(0)  # call by call: sizes every buffer, uploads the expert tables
             self.graphs = [] if not self._record_step_graphs() else self.graphs
