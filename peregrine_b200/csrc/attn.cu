@@ -165,7 +165,7 @@ struct NormRopeLaunch {
     }
 };
 
-// Problems with more row vectors than this go to the tensor-memory kernel, whose tiles have 128 rows.
+// Problems with more row vectors than this go to the tensor-memory kernel, whose tiles have 128 rows (both sides: kAtMany).
 constexpr int kTcRows = kAtMany;
 
 // Row tile of the split kernel.

@@ -24,7 +24,18 @@ constexpr int kAtKeys = 64;      // keys of a tile
 constexpr int kAtThreads = 160;  // 4 warps with 16 keys of a tile each, one that issues the copies
 constexpr int kAtCombine = 128;
 constexpr int kTcKeys = 64;  // keys of a tile of the tensor-memory kernel
-constexpr int kAtMany = 16;     // row vectors of a problem up to which the joining launch adds up the weights itself
+// Row vectors of a problem up to which attn_split_kernel takes it, and the joining launch adds up the weights itself.  us of a
+// call with 4 key heads, bf16, fp32 out, by that kernel / by the one on tensor memory:
+//                              12 row vectors     20 row vectors
+//   D = 64,  1 x 20000 slots    17.5 / 24.3        19.1 / 24.3
+//   D = 64,  8 x 4000           15.4 / 19.9        18.7 / 20.2
+//   D = 128, 1 x 20000          24.7 / 27.1        27.6 / 27.6
+//   D = 128, 8 x 4000           24.9 / 22.9        29.8 / 23.2
+//   D = 256, 1 x 20000          43.9 / 28.7        71.3 / 28.8
+//   D = 256, 8 x 4000           51.5 / 27.3        71.9 / 29.4
+// and of 12 and 20 rows behind 2000 keys (D = 128): 11.5 / 15.6, 14.7 / 16.2.  The border suits D = 128; at D = 256, where a row tile of
+// 16 takes all 255 registers and spills 500 bytes, up to 8 (26.1 us for 8 x 4000) the split kernel keeps up, beyond not.
+constexpr int kAtMany = 16;
 constexpr int kAtChunk = 1024;  // slots whose weights one CTA adds up
 
 struct AttnArgs {
@@ -728,8 +739,9 @@ __device__ __forceinline__ void attn_weigh(float (&sum)[4], const float4 &x, con
 }
 
 // Joins the partials.  The first `row_ctas` CTAs take 4 / WPR row vectors each, WPR warps to one (4 where there are too few
-// row vectors to fill the device with a warp each: below 16 an SM; 24.8 instead of 29.0 us for a call of 1120 row vectors, 91.9
-// instead of 93.6 for one of 2048); with acc and up to kAtMany row vectors a problem, further CTAs take 1024 slots of one
+// row vectors to fill the device with a warp each: below 16 an SM.  A call of 16, 24, 36 and 38 rows x 64 heads behind 8192 keys
+// takes 29.3, 37.2, 54.1 and 54.5 us with four warps, 34.1, 37.8, 51.1 and 51.3 with one; the last two lie on either side
+// of the border); with acc and up to kAtMany row vectors a problem, further CTAs take 1024 slots of one
 // (sequence, kv head) each.  What bounds it is a chain of latencies (CTAs of a unit, statistics, partials), so all that does
 // not hang on the launches before comes ahead of the wait for them, and eight partials of a warp are under way together.
 template <int D, bool BF16, int WPR>

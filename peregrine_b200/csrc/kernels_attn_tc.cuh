@@ -4,16 +4,19 @@
 //     S = Q K^T (tensor memory) -> weights 2^(x - m), written over S as the A operand -> O += P V (tensor memory)
 // Two threads own a row (its TMEM lane), 32 columns of a tile each: with one, two warps a scheduler form the weights and hide
 // little of each other's latencies (53.5 us instead of 51.7 for the call below).  The two row tiles
-// alternate: while one's weights are formed the tensor unit works for the other.  A 128 x 128 tile takes the tensor unit
-// 2 x 512 cycles (D = 128) and the exponential unit (16 a cycle) 1024, so neither can wait for the other; S has two buffers
-// where they fit, so that the next scores are there when a tile's weights are done.  O is rescaled
-// only when a row's maximum has grown by 2^8 since it was last set: m only has to keep weights in range, and cancels in
-// O / l.  With at most 128 row vectors both tiles hold the same ones and the key tiles go to them in turn.  D = 256 has
+// alternate: while one's weights are formed the tensor unit works for the other.  A step of 64 keys x 256 rows (D = 128) takes the
+// tensor unit 1280 cycles at the least (a 64-column product of the scores reads its operands from shared memory for 48 cycles and
+// multiplies for 32; the second product 64) and the exponential unit (16 a cycle) 1024, so neither can wait for the other; S has
+// two buffers where they fit, so that the next scores are there when a tile's weights are done.  O is rescaled only when a
+// row's maximum has grown by 2^8 since it was last set: m only has to keep weights in range, and cancels in O / l.  With at most 128 row vectors both tiles hold the same ones and the key tiles go to them in turn.  D = 256 has
 // no room for a second O: there one tile alternates between two S.
 //
-// Measured: 32 rows x 64 heads behind 32768 keys (8 key heads of 128, bf16 out) 48 us, 716 TFLOP/s of the 1669 that cuBLAS
-// reaches; 0.77 us a step of 64 keys x 256 rows, 1430 cycles of the 1280 that the products need (a 64-column product reads
-// its operands from shared memory for 48 cycles and multiplies for 32).  A CTA's start and end take about 9 us.
+// Measured: 32 rows x 64 heads behind 32768 keys (8 key heads of 128, bf16 out, keys from HBM) 46 us, 747 TFLOP/s of the 1669
+// that cuBLAS reaches.  A CTA's 43 us (the slowest's 45): 2.1 until its place on the line is known, 3.1 until the first scores
+// are there, 33.5 for 28 steps, 3.2 until its partial result is written, 1.1 until the last warp of it is done.  The first step takes
+// 2.8 us (the second tile is asked for when the query vectors are there), the others 1.10 us, 1950 cycles at 1.77 GHz: the
+// issuing thread waits about 270 of them for weights and stands in the tensor unit's full queue for nearly all others; a
+// step's keys and values are there when it asks (2.9 TB/s).
 //
 // Only the last tiles of a problem have keys that some row does not see; there, S is masked after it was read, and what the
 // values of such keys may hold is taken out of the tile in shared memory before the product (0 x inf is not 0).  Work is
@@ -24,9 +27,12 @@
 namespace pgb {
 
 // Tiles that a change of the problem costs a CTA (query vectors, first and last tile, its partial result): on the line every
-// (problem, row tile) begins with so many empty ones.
+// (problem, row tile) begins with so many empty ones.  With 4, 8 and 16: 5 drafts of 8 rows (28 heads of 64) 23.7, 24.8 and 26.5 us,
+// 64 x 8 rows (32 heads of 128) over 300 slots 52.5, 54.6 and 59.1, over 2000 slots 119.9, 117.8 and 124.2, the call above the same.
 constexpr int kTcEmpty = 8;
-constexpr int kTcLeast = 4;  // tiles (empty ones too) of a CTA at least
+// Tiles (empty ones too) of a CTA at least.  With 1, 4 and 8: 8 rows over 3000 slots (4 key heads of 128) 18.0, 16.9 and 21.6 us, 64 x 64 heads
+// behind 32768 keys 87.8, 86.7 and 86.8; but 64 rows over 1500 slots (4 key heads of 128) 17.1, 23.5 and 31.0.
+constexpr int kTcLeast = 4;
 
 template <int D, bool BF16, bool F32>
 struct TcShape {
