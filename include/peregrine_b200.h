@@ -277,7 +277,9 @@ int coli_cuda_pipe_qk_norm_rope(int device, void *q_out, const float *qkv_dev, l
  * already stored at base_dev[b] + i.  Row i sees the prefix, its sequence's slots below base_dev[b], and of the
  * new slots base_dev[b] + j those with bit j of mask_dev[s] set (mask_dev NULL: j <= i); never a slot at or
  * past own->cap.  out [S, H, D] = softmax(scale q.k) v over what the row sees, fp32 (out_f32 = 1) or the cache's
- * dtype (0); a row that sees nothing is 0; rows of a sequence with base_dev[b] < 0 are left as they were.
+ * dtype (0); a row that sees nothing is 0; rows of a sequence with base_dev[b] < 0 are left as they were.  An infinite or
+ * NaN value makes its one element infinite or NaN in the rows that see it (not always the infinity it was: a weight's
+ * terms may be zero or of either sign) and changes nothing else.
  * When own->acc is set, acc[b, kv head, slot] grows by the softmax weights the slot received from the rows and
  * heads of its group.  Products of 16-bit values are summed in fp32, softmax statistics are fp32.  With out_f32 a
  * weight w enters the second product within 2^-21 w; from an f16 cache within 2^-30 of the row's largest weight where

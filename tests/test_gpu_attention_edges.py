@@ -178,3 +178,47 @@ def test_small_weights_beside_a_large_one(dev, T, G, r, Tp):
         tiny = 1.5 * count[:, :, None] * 2.0 ** -30 if T == "f16" else 0.0
         off = np.abs(f64(out) - want)
         assert np.all(off <= want * (each + 2.0 ** -21) + tiny), (x, float((off / want).max()))
+
+
+@pytest.mark.parametrize("n, r, G, Kv, D, T, Tp, out_f32", [
+    (3, 1, 4, 2, 64, "bf16", 150, True), (2, 3, 4, 2, 128, "f16", 0, False), (5, 9, 4, 1, 256, "bf16", 0, True),
+    (4, 12, 12, 2, 64, "f16", 90, True), (24, 1, 8, 2, 128, "bf16", 400, False), (1, 40, 5, 2, 128, "bf16", 70, True),
+])
+def test_infinite_values_stay_in_the_elements_that_see_them(dev, n, r, G, Kv, D, T, Tp, out_f32):
+    """In the prefix, among the slots that all rows of a sequence see, and among the new ones, of which masks hide some."""
+    rng = np.random.default_rng(n + D)
+    H, S, cap = G * Kv, n * r, r + 150
+    q = torch.from_numpy(rng.standard_normal((S, H, D), dtype=np.float32)).to(TYPES[T]).cuda()
+    k, v = (ref.cache(rng, n, Kv, cap, D, T) for _ in range(2))
+    pk, pv = (ref.cache(rng, 1, Kv, max(Tp, 1), D, T) for _ in range(2))
+    base = rng.integers(1, cap - r + 1, n)
+    bits = rng.integers(0, 1 << min(r, 62), S).astype(np.uint64)
+    odd = np.array([np.inf, -np.inf, np.nan])
+    for b in range(n):
+        for _ in range(3):
+            low = 0 if rng.random() < 0.4 else base[b]
+            v[b, rng.integers(Kv), rng.integers(low, base[b] + r), rng.integers(D)] = float(rng.choice(odd))
+        k[b, :, base[b] + r:], v[b, :, base[b] + r:] = float("nan"), float("-inf")
+    if Tp:
+        pv[0, 0, rng.integers(Tp), 5] = float("inf")
+    clean, pclean = (torch.where(torch.isfinite(x), x, 0.0) for x in (v, pv))
+    out = torch.zeros((S, H, D), dtype=torch.float32 if out_f32 else TYPES[T], device="cuda")
+    own, pre, bdev, mask = ref.view(k, v, T), ref.view(pk, pv, T), i32(base), torch.from_numpy(bits.view(np.int64)).cuda()
+    need = at.attention_workspace(0, S, H, own, Tp, r)
+    work = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    at.attention(0, out.data_ptr(), q.data_ptr(), S, H, own, bdev.data_ptr(), D ** -0.5, work.data_ptr(), need, rows_per_seq=r,
+                 prefix=pre if Tp else None, prefix_len=Tp, mask=mask.data_ptr(), out_f32=out_f32)
+    ref.done()
+    got, prefix = f64(out), (f64(pk)[0], f64(pclean)[0]) if Tp else (None, None)
+    want, _, gam, mag = ref.attend(f64(q), f64(k), f64(clean), base, r, D ** -0.5, *prefix, mask=bits)
+    tol = ref.bound(gam, mag, Tp + cap + 64, want, T, out_f32)
+    hit = np.zeros((S, Kv, D), bool)  # what an odd value is seen by
+    for s in range(S):
+        seen = ref.visible(cap, base[s // r], s % r, r, bits[s])
+        hit[s] = (~np.isfinite(f64(v[s // r])) & seen[None, :, None]).any(1)
+        if Tp:
+            hit[s] |= (~np.isfinite(f64(pv[0]))).any(1)
+    hit = np.repeat(hit, G, 1)
+    assert hit.any() and np.array_equal(~np.isfinite(got), hit)
+    assert np.all((np.abs(got - want) <= tol)[~hit])
