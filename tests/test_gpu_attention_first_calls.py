@@ -1,10 +1,12 @@
 """The attention operators' first calls in a process are recorded ones."""
+import os
 import subprocess
 import sys
 
 import pytest
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 SCRIPT = r"""
 import ctypes as C
@@ -63,5 +65,5 @@ print("recorded")
 
 
 def test_the_first_calls_of_a_process_may_be_recorded_ones():
-    done = subprocess.run([sys.executable, "-c", SCRIPT], capture_output=True, text=True, timeout=300)
+    done = subprocess.run([sys.executable, "-c", SCRIPT], capture_output=True, text=True, timeout=300, cwd=ROOT)
     assert done.returncode == 0 and "recorded" in done.stdout, done.stdout + done.stderr

@@ -1,10 +1,12 @@
 """Two decode stacks on one device share its scratch."""
+import os
 import subprocess
 import sys
 
 import pytest
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 # a process of its own: the scratch has not grown before
 SCRIPT = r"""
@@ -37,5 +39,5 @@ print("the same")
 
 
 def test_recorded_steps_follow_scratch_that_a_wider_stack_has_moved():
-    done = subprocess.run([sys.executable, "-c", SCRIPT], capture_output=True, text=True, timeout=300)
+    done = subprocess.run([sys.executable, "-c", SCRIPT], capture_output=True, text=True, timeout=300, cwd=ROOT)
     assert done.returncode == 0 and "the same" in done.stdout, done.stdout + done.stderr
